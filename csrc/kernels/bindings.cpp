@@ -20,6 +20,16 @@ void rms_norm(torch::Tensor out, torch::Tensor x, torch::Tensor w, double eps);
 void fused_add_rms_norm(torch::Tensor x, torch::Tensor residual, torch::Tensor w, double eps);
 void rope_kv_write(torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin, torch::Tensor k_cache,
                    torch::Tensor v_cache, torch::Tensor slot_mapping, int64_t hq, int64_t hk, int64_t d, int64_t rot);
+// 4-bit KV cache (kv_fp4_bindings.cpp)
+void rope_kv_write_fp4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin,
+                       torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots, int64_t hq, int64_t hk,
+                       int64_t d, int64_t rot, double k_scale, double v_scale);
+void kv_fp4_read(torch::Tensor k_out, torch::Tensor v_out, torch::Tensor k_cache, torch::Tensor v_cache,
+                 torch::Tensor slots, int64_t d, double k_scale, double v_scale);
+void paged_attention_fp4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
+                         torch::Tensor block_tables, torch::Tensor seq_lens, torch::Tensor q_start, int64_t hq,
+                         int64_t d, double scale, int64_t max_q_len, double k_scale, double v_scale, bool invariant);
+void copy_kv_pages(const std::vector<torch::Tensor>& caches, torch::Tensor src, torch::Tensor dst);
 void silu_mul(torch::Tensor out, torch::Tensor x);
 void embedding(torch::Tensor out, torch::Tensor ids, torch::Tensor table);
 void argmax_rows(torch::Tensor out, torch::Tensor logits);
@@ -1088,6 +1098,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm", &rms_norm);
   m.def("fused_add_rms_norm", &fused_add_rms_norm);
   m.def("rope_kv_write", &rope_kv_write);
+  m.def("rope_kv_write_fp4", &rope_kv_write_fp4);
+  m.def("kv_fp4_read", &kv_fp4_read);
+  m.def("paged_attention_fp4", &paged_attention_fp4);
+  m.def("copy_kv_pages", &copy_kv_pages);
   m.def("silu_mul", &silu_mul);
   m.def("embedding", &embedding);
   m.def("argmax_rows", &argmax_rows);

@@ -1,0 +1,241 @@
+// Python bindings of the 4-bit KV cache: writer, reader, paged attention, page copies.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <map>
+#include <mutex>
+#include <tuple>
+#include <vector>
+
+#include "kv_fp4.h"
+#include "paged_attention_fp4.h"
+
+namespace {
+
+constexpr double kLog2e = 1.4426950408889634;
+
+int64_t page_bytes(int64_t d) { return 64 * (d / 2 + d / 16); }
+
+void check_dim(int64_t d, const char* who) {
+  TORCH_CHECK(d == 64 || d == 128 || d == 256, who, ": head_dim 64, 128 or 256, got ", d);
+}
+
+void check_cache(const torch::Tensor& k, const torch::Tensor& v, int64_t d, const char* who) {
+  for (const torch::Tensor* c : {&k, &v})
+    TORCH_CHECK(c->is_cuda() && c->scalar_type() == at::kByte && c->dim() == 3 && c->is_contiguous() &&
+                    c->size(2) == page_bytes(d),
+                who, ": caches uint8 [num_blocks, kv_heads, ", page_bytes(d), "] contiguous on a CUDA device");
+  TORCH_CHECK(k.sizes() == v.sizes(), who, ": key and value caches of one shape");
+  TORCH_CHECK(k.size(0) > 0 && k.size(0) <= 0x7fffffff, who, ": 1 .. 2^31 - 1 blocks");
+}
+
+void check_index(const torch::Tensor& t, at::ScalarType type, int64_t dim, const torch::Tensor& like, const char* who,
+                 const char* name) {
+  TORCH_CHECK(t.scalar_type() == type && t.dim() == dim && t.device() == like.device(), who, ": ", name, " must be ",
+              c10::toString(type), " with ", dim, " dimension(s) on ", like.device());
+  TORCH_CHECK(t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1, who, ": ", name, " must have unit stride");
+}
+
+void check_rows(const torch::Tensor& t, int64_t width, const torch::Tensor& like, const char* who, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.device() == like.device(), who,
+              ": ", name, " must be bf16 [tokens, width] on ", like.device());
+  TORCH_CHECK(t.size(1) >= width && (t.size(1) <= 1 || t.stride(1) == 1), who, ": ", name, " needs ", width,
+              " columns of unit stride");
+  TORCH_CHECK(t.size(0) == 0 || (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                                 (t.size(0) == 1 || t.stride(0) % 8 == 0)),
+              who, ": ", name, " rows must be 16-byte aligned");
+}
+
+// Partial results and tickets of the split units, one set per stream: calls on a stream follow one another, calls on
+// two streams may overlap.  A stream under capture gets a set of its own for that capture, so that a replay never
+// shares one with eager calls; it lives in the graph's pool, and its tickets are zeroed by a node of the graph.
+struct Scratch {
+  torch::Tensor part, tickets;
+};
+
+Scratch scratch(const torch::Tensor& like, cudaStream_t stream, int64_t floats, int64_t ctas) {
+  static std::mutex mu;
+  static auto* eager = new std::map<std::pair<int, cudaStream_t>, Scratch>();  // never destroyed: outlives CUDA
+  static auto* captured = new std::map<int, std::pair<unsigned long long, Scratch>>();
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  TORCH_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id) == cudaSuccess, "paged_attention_fp4: stream capture state");
+  std::lock_guard<std::mutex> lock(mu);
+  const int dev = like.get_device();
+  Scratch* s;
+  if (status == cudaStreamCaptureStatusActive) {
+    auto& slot = (*captured)[dev];
+    if (slot.first != id) slot = {id, Scratch{}};
+    s = &slot.second;
+  } else {
+    s = &(*eager)[{dev, stream}];
+  }
+  if (!s->part.defined() || s->part.numel() < floats)
+    s->part = torch::empty({floats}, like.options().dtype(at::kFloat));
+  if (!s->tickets.defined() || s->tickets.numel() < ctas)
+    s->tickets = torch::zeros({ctas}, like.options().dtype(at::kInt));
+  return *s;
+}
+
+}  // namespace
+
+void rope_kv_write_fp4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin,
+                       torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots, int64_t hq, int64_t hk,
+                       int64_t d, int64_t rot, double k_scale, double v_scale) {
+  const char* who = "rope_kv_write_fp4";
+  check_dim(d, who);
+  check_cache(k_cache, v_cache, d, who);
+  TORCH_CHECK(hq > 0 && hk > 0 && k_cache.size(1) == hk, who, ": the caches hold ", k_cache.size(1), " kv heads, not ", hk);
+  check_rows(qkv, (hq + 2 * hk) * d, k_cache, who, "qkv");
+  check_rows(q_out, hq * d, k_cache, who, "q_out");
+  TORCH_CHECK(q_out.size(0) == qkv.size(0), who, ": one q_out row per token");
+  TORCH_CHECK(!q_out.is_alias_of(qkv), who, ": q_out must not share qkv's memory (a rotation reads both halves)");
+  check_index(positions, at::kLong, 1, k_cache, who, "positions");
+  check_index(slots, at::kLong, 1, k_cache, who, "slot_mapping");
+  TORCH_CHECK(positions.numel() == qkv.size(0) && slots.numel() == qkv.size(0), who, ": one position and slot per token");
+  TORCH_CHECK(rot >= 0 && rot <= d && rot % 2 == 0, who, ": rot must be even and at most head_dim");
+  TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 2 && cos_sin.size(1) == rot &&
+                  cos_sin.is_contiguous() && cos_sin.device() == k_cache.device() && cos_sin.size(0) > 0,
+              who, ": cos_sin must be f32 [positions, rot] contiguous");
+  TORCH_CHECK(k_scale > 0 && v_scale > 0, who, ": cache scales must be positive");
+  if (qkv.size(0) == 0) return;
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  KvFp4WriteParams p{};
+  p.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv.data_ptr());
+  p.qkv_stride = qkv.size(0) == 1 ? 0 : qkv.stride(0);
+  p.q_out = reinterpret_cast<__nv_bfloat16*>(q_out.data_ptr());
+  p.q_stride = qkv.size(0) == 1 ? 0 : q_out.stride(0);
+  p.positions = positions.data_ptr<int64_t>();
+  p.cos_sin = cos_sin.data_ptr<float>();
+  p.max_pos = cos_sin.size(0);
+  p.slots = slots.data_ptr<int64_t>();
+  p.k_cache = k_cache.data_ptr<uint8_t>();
+  p.v_cache = v_cache.data_ptr<uint8_t>();
+  p.num_tokens = qkv.size(0);
+  p.num_slots = k_cache.size(0) * 64;
+  p.hq = static_cast<int>(hq);
+  p.hk = static_cast<int>(hk);
+  p.rot = static_cast<int>(rot);
+  p.k_inv = static_cast<float>(1.0 / k_scale);
+  p.v_inv = static_cast<float>(1.0 / v_scale);
+  const int r = sh_kv_fp4_write(&p, static_cast<int>(d), at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(r == 0, "sh_kv_fp4_write failed with code ", r);
+}
+
+void kv_fp4_read(torch::Tensor k_out, torch::Tensor v_out, torch::Tensor k_cache, torch::Tensor v_cache,
+                 torch::Tensor slots, int64_t d, double k_scale, double v_scale) {
+  const char* who = "kv_fp4_read";
+  check_dim(d, who);
+  check_cache(k_cache, v_cache, d, who);
+  check_index(slots, at::kLong, 1, k_cache, who, "slots");
+  for (const torch::Tensor* o : {&k_out, &v_out})
+    TORCH_CHECK(o->scalar_type() == at::kBFloat16 && o->is_contiguous() && o->device() == k_cache.device() &&
+                    o->dim() == 3 && o->size(0) == slots.numel() && o->size(1) == k_cache.size(1) && o->size(2) == d &&
+                    reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0,
+                who, ": outputs bf16 [slots, kv_heads, head_dim] contiguous");
+  if (slots.numel() == 0) return;
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  KvFp4ReadParams p{};
+  p.k_cache = k_cache.data_ptr<uint8_t>();
+  p.v_cache = v_cache.data_ptr<uint8_t>();
+  p.k_out = reinterpret_cast<__nv_bfloat16*>(k_out.data_ptr());
+  p.v_out = reinterpret_cast<__nv_bfloat16*>(v_out.data_ptr());
+  p.slots = slots.data_ptr<int64_t>();
+  p.n = slots.numel();
+  p.num_slots = k_cache.size(0) * 64;
+  p.hk = static_cast<int>(k_cache.size(1));
+  p.k_scale = static_cast<float>(k_scale);
+  p.v_scale = static_cast<float>(v_scale);
+  const int r = sh_kv_fp4_read(&p, static_cast<int>(d), at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(r == 0, "sh_kv_fp4_read failed with code ", r);
+}
+
+void paged_attention_fp4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
+                         torch::Tensor block_tables, torch::Tensor seq_lens, torch::Tensor q_start, int64_t hq,
+                         int64_t d, double scale, int64_t max_q_len, double k_scale, double v_scale, bool invariant) {
+  const char* who = "paged_attention_fp4";
+  check_dim(d, who);
+  check_cache(k_cache, v_cache, d, who);
+  const int64_t hk = k_cache.size(1), B = seq_lens.numel();
+  TORCH_CHECK(hk > 0 && hq > 0 && hq % hk == 0, who, ": ", hq, " query heads over ", hk, " kv heads");
+  check_rows(q, hq * d, k_cache, who, "q");
+  check_rows(out, hq * d, k_cache, who, "out");
+  TORCH_CHECK(out.size(0) == q.size(0), who, ": one out row per q row");
+  check_index(block_tables, at::kInt, 2, k_cache, who, "block_tables");
+  check_index(seq_lens, at::kLong, 1, k_cache, who, "seq_lens");
+  check_index(q_start, at::kLong, 1, k_cache, who, "q_start");
+  TORCH_CHECK(q_start.numel() == B + 1 && block_tables.size(0) == B, who, ": q_start of ", B + 1, " and block_tables of ",
+              B, " rows for ", B, " lengths");
+  TORCH_CHECK(max_q_len >= 1, who, ": max_q_len must be at least 1");
+  TORCH_CHECK(k_scale > 0 && v_scale > 0, who, ": cache scales must be positive");
+  if (q.size(0) == 0 || B == 0) return;
+  TORCH_CHECK(block_tables.size(1) > 0, who, ": block_tables without columns");
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  AttnFp4Params p{};
+  p.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  p.out_stride = out.size(0) == 1 ? 0 : out.stride(0);
+  p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
+  p.q_stride = q.size(0) == 1 ? 0 : q.stride(0);
+  p.k_cache = k_cache.data_ptr<uint8_t>();
+  p.v_cache = v_cache.data_ptr<uint8_t>();
+  p.block_tables = block_tables.data_ptr<int32_t>();
+  p.bt_stride = block_tables.stride(0);
+  p.seq_lens = seq_lens.data_ptr<int64_t>();
+  p.q_start = q_start.data_ptr<int64_t>();
+  p.num_tokens = q.size(0);
+  p.B = static_cast<int>(B);
+  p.hq = static_cast<int>(hq);
+  p.hk = static_cast<int>(hk);
+  p.num_blocks = static_cast<int>(k_cache.size(0));
+  p.bt_cols = static_cast<int>(std::min<int64_t>(block_tables.size(1), 1 << 25));
+  p.whole_units = invariant ? 1 : 0;
+  p.scale_log2 = static_cast<float>(scale * k_scale * kLog2e);
+  p.v_scale = static_cast<float>(v_scale);
+  // Rows of one kv head that a CTA holds: as many as the longest query has, up to what its registers carry.
+  const int64_t rows = std::min<int64_t>(max_q_len, 64) * (hq / hk);
+  const int tile = static_cast<int>(std::min<int64_t>((rows + 7) / 8 * 8, d == 256 ? 16 : 32));
+  const int ctas = sh_paged_attention_fp4_ctas(static_cast<int>(d), tile);
+  TORCH_CHECK(ctas > 0, who, ": no CUDA device");
+  const Scratch s = scratch(k_cache, stream, sh_paged_attention_fp4_workspace(static_cast<int>(d), tile), ctas);
+  p.part_o = s.part.data_ptr<float>();
+  p.tickets = reinterpret_cast<unsigned*>(s.tickets.data_ptr<int>());
+  const int r = sh_paged_attention_fp4(&p, static_cast<int>(d), tile, stream);
+  TORCH_CHECK(r == 0, "sh_paged_attention_fp4 failed with code ", r);
+}
+
+void copy_kv_pages(const std::vector<torch::Tensor>& caches, torch::Tensor src, torch::Tensor dst) {
+  const char* who = "copy_kv_pages";
+  TORCH_CHECK(!caches.empty() && caches[0].is_cuda(), who, ": at least one CUDA cache tensor");
+  check_index(src, at::kLong, 1, caches[0], who, "src");
+  check_index(dst, at::kLong, 1, caches[0], who, "dst");
+  TORCH_CHECK(src.numel() == dst.numel(), who, ": ", src.numel(), " sources for ", dst.numel(), " destinations");
+  for (const torch::Tensor& c : caches) {
+    TORCH_CHECK(c.device() == caches[0].device() && c.dim() >= 2 && c.is_contiguous(), who,
+                ": cache tensors [num_blocks, ...] contiguous on one device");
+    TORCH_CHECK(c.numel() == 0 || ((c.numel() / c.size(0)) * c.element_size() % 16 == 0 &&
+                                   reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0),
+                who, ": pages must be multiples of 16 bytes and 16-byte aligned");
+  }
+  if (src.numel() == 0) return;
+  const c10::cuda::CUDAGuard guard(caches[0].device());
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  for (size_t at = 0; at < caches.size(); at += SH_KV_COPY_MAX_TENSORS) {
+    KvCopyParams p{};
+    p.src = src.data_ptr<int64_t>();
+    p.dst = dst.data_ptr<int64_t>();
+    p.n = src.numel();
+    for (size_t i = at; i < caches.size() && i < at + SH_KV_COPY_MAX_TENSORS; ++i) {
+      const torch::Tensor& c = caches[i];
+      if (c.numel() == 0) continue;
+      p.base[p.tensors] = static_cast<uint8_t*>(c.data_ptr());
+      p.page_bytes[p.tensors] = (c.numel() / c.size(0)) * c.element_size();
+      p.pages[p.tensors] = c.size(0);
+      ++p.tensors;
+    }
+    const int r = sh_kv_copy_pages(&p, stream);
+    TORCH_CHECK(r == 0, "sh_kv_copy_pages failed with code ", r);
+  }
+}

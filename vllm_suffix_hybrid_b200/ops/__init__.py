@@ -173,6 +173,80 @@ def paged_attention(out, q, k_cache, v_cache, block_tables, seq_lens, q_start, t
     return out
 
 
+# ----------------------------------------------------------------------------- 4-bit KV cache (GQA)
+def kv_fp4_cache_shape(num_blocks: int, kv_heads: int, d: int) -> tuple:
+    """Shape of a 4-bit cache tensor (uint8), one for the keys and one for the values: a page per (block, head)
+    holds its 64 tokens' codes (two e2m1 codes a byte, even dimension in the low nibble), then their e4m3 scales,
+    one per 16 dimensions."""
+    if d not in (64, 128, 256):
+        raise ValueError(f"the 4-bit KV cache needs head_dim 64, 128 or 256, got {d}")
+    return (num_blocks, kv_heads, 64 * (d // 2 + d // 16))
+
+
+def rope_kv_write_fp4(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, hq, hk, d, rot=None,
+                      k_scale: float = 1.0, v_scale: float = 1.0, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """RoPE of the new tokens' queries and keys, keys and values quantised into the 4-bit pages of their slots.
+
+    qkv [T, (hq + 2 hk) D] is only read; the rotated queries [T, hq D] are returned (into q_out when given).  A row
+    with a slot outside the cache (< 0: padding) caches nothing; two rows of one call must not share a slot.  The
+    caches hold x / k_scale and x / v_scale: e2m1 codes times e4m3 scales of 16 dimensions, from 2^-10 to 2688."""
+    rot = d if rot is None else rot
+    if not _cuda(qkv):
+        q = ref.rope_kv_write_fp4(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, hq, hk, d, rot, k_scale,
+                                  v_scale)
+        return q if q_out is None else q_out.copy_(q)
+    if q_out is None:
+        q_out = torch.empty(qkv.shape[0], hq * d, dtype=qkv.dtype, device=qkv.device)
+    native().rope_kv_write_fp4(q_out, qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, hq, hk, d, rot, k_scale,
+                               v_scale)
+    return q_out
+
+
+def kv_fp4_read(k_cache, v_cache, slots, d, k_scale: float = 1.0, v_scale: float = 1.0):
+    """The cached keys and values of `slots` [n] as (k, v) [n, hk, D] in bf16 (fp32 on the CPU); zeros for a slot
+    outside the cache."""
+    if not _cuda(k_cache):
+        return ref.kv_fp4_read(k_cache, slots, d, k_scale), ref.kv_fp4_read(v_cache, slots, d, v_scale)
+    k = torch.empty(slots.shape[0], k_cache.shape[1], d, dtype=torch.bfloat16, device=k_cache.device)
+    v = torch.empty_like(k)
+    native().kv_fp4_read(k, v, k_cache, v_cache, slots, d, k_scale, v_scale)
+    return k, v
+
+
+def paged_attention_fp4(out, q, k_cache, v_cache, block_tables, seq_lens, q_start, hq, d, scale, max_q_len: int,
+                        k_scale: float = 1.0, v_scale: float = 1.0):
+    """out[T, hq*D] <- causal attention of q [T, hq*D] over the 4-bit paged cache.
+
+    seq_lens [B] counts the new tokens; q_start [B + 1] their rows; max_q_len is the longest of them (it picks the
+    kernel's row tile, a smaller number stays correct).  Rows that see no key are zero.  No plan, split count or
+    length is needed on the host.  In batch-invariant mode (SH_BATCH_INVARIANT=1) a row's result does not depend on
+    the other rows of the call."""
+    if not _cuda(q):
+        t = q.shape[0]
+        out.view(t, hq, d).copy_(ref.paged_attention_fp4(q[:, : hq * d].reshape(t, hq, d), k_cache, v_cache, block_tables,
+                                                         seq_lens, q_start, hq, d, scale, k_scale, v_scale))
+        return out
+    native().paged_attention_fp4(out, q, k_cache, v_cache, block_tables, seq_lens, q_start, hq, d, scale, max_q_len,
+                                 k_scale, v_scale, os.environ.get("SH_BATCH_INVARIANT", "0") == "1")
+    return out
+
+
+def copy_kv_pages(caches, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """cache[dst[i]] = cache[src[i]] for every tensor [num_blocks, ...] of `caches` (one launch for up to 128).
+
+    src, dst: int64 [n] block ids on the caches' device; a pair with an id outside a tensor is skipped.  No id may
+    be a destination twice, or both a source and a destination (the copies run in no order)."""
+    caches = list(caches)
+    if not caches:
+        return
+    if not _cuda(caches[0]):
+        for c in caches:
+            ok = (src >= 0) & (dst >= 0) & (src < c.shape[0]) & (dst < c.shape[0])
+            c[dst[ok]] = c[src[ok]]
+        return
+    native().copy_kv_pages(caches, src, dst)
+
+
 # ----------------------------------------------------------------------------- activations / gather
 def silu_mul(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     if not _cuda(x):

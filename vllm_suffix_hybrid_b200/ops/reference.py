@@ -151,6 +151,87 @@ def paged_attention(q, k_cache, v_cache, block_tables, seq_lens, q_start, hq, sc
     return out
 
 
+# ----------------------------------------------------------------------------- 4-bit KV cache (GQA)
+def kv_fp4_quantize(x: torch.Tensor):
+    """x [..., D] -> (packed codes uint8 [..., D/2], e4m3 scales as bytes [..., D/16]).
+
+    Per 16 values s = e4m3(clamp(max|x| / 6, 2^-9, 448)), code = e2m1(x / s), both to nearest even and saturating
+    (an infinity becomes the largest code; a NaN too, and it does not count in the maximum)."""
+    xf = x.float()
+    b = xf.reshape(*xf.shape[:-1], -1, 16)
+    amax = torch.where(torch.isnan(b), torch.zeros_like(b), b.abs()).amax(-1)
+    s = (amax / torch.full((), 6.0, device=x.device)).clamp(2.0 ** -9, 448.0).to(torch.float8_e4m3fn)
+    y = b / s.float()[..., None]
+    codes = torch.where(torch.isnan(y), torch.full_like(y, 7).to(torch.uint8), e2m1_codes(y))
+    # e2m1_codes keeps the sign of negative values; a negative zero has one as well
+    codes = torch.where(torch.signbit(b) & ~torch.isnan(b), codes | 8, codes).reshape(xf.shape)
+    return codes[..., 0::2] | (codes[..., 1::2] << 4), s.view(torch.uint8)
+
+
+def kv_fp4_dequantize(packed: torch.Tensor, scales: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """fp32 values [..., D] of packed codes and scale bytes (times the cache's scale)."""
+    codes = torch.stack([packed & 15, packed >> 4], -1).flatten(-2).long()
+    mag = E2M1.to(packed.device)[codes & 7]
+    v = torch.where(codes & 8 > 0, -mag, mag).unflatten(-1, (-1, 16))
+    return (v * scales.view(torch.float8_e4m3fn).float()[..., None]).flatten(-2) * scale
+
+
+def _kv_fp4_views(cache: torch.Tensor, d: int):
+    """(codes [blocks, hk, 64, D/2], scale bytes [blocks, hk, 64, D/16]) views of a cache tensor."""
+    split = 64 * d // 2
+    return cache[..., :split].unflatten(-1, (64, -1)), cache[..., split:].unflatten(-1, (64, -1))
+
+
+def rope_kv_write_fp4(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, hq, hk, d, rot, k_scale, v_scale):
+    """Rotated queries [T, hq*D]; the rotated keys and the values go quantised into their slots."""
+    t = qkv.shape[0]
+    x = qkv[:, : (hq + 2 * hk) * d].to(torch.float32, copy=True).reshape(t, hq + 2 * hk, d)
+    if rot:
+        x[:, : hq + hk] = apply_rope(x[:, : hq + hk], positions, cos_sin)
+    ok = (slot_mapping >= 0) & (slot_mapping < k_cache.shape[0] * 64)
+    blk, off = slot_mapping[ok] // 64, slot_mapping[ok] % 64
+    for cache, rows, scale in ((k_cache, x[:, hq:hq + hk], k_scale), (v_cache, x[:, hq + hk:], v_scale)):
+        inv = torch.tensor(1.0 / scale, dtype=torch.float32)
+        packed, sc = kv_fp4_quantize(rows[ok] * inv)
+        codes, scales = _kv_fp4_views(cache, d)
+        codes[blk, :, off] = packed
+        scales[blk, :, off] = sc
+    return x[:, :hq].reshape(t, hq * d).to(qkv.dtype)
+
+
+def kv_fp4_read(cache, slots, d, scale):
+    """fp32 rows [n, hk, D] of the slots; zeros for a slot outside the cache."""
+    ok = (slots >= 0) & (slots < cache.shape[0] * 64)
+    at = torch.where(ok, slots, torch.zeros_like(slots))
+    codes, scales = _kv_fp4_views(cache, d)
+    x = kv_fp4_dequantize(codes[at // 64, :, at % 64], scales[at // 64, :, at % 64], scale)
+    return torch.where(ok[:, None, None], x, torch.zeros_like(x))
+
+
+def paged_attention_fp4(q, k_cache, v_cache, block_tables, seq_lens, q_start, hq, d, scale, k_scale, v_scale):
+    """q: [T, hq, D] -> [T, hq, D]; rows that see no key are zero."""
+    hk = k_cache.shape[1]
+    out = torch.zeros_like(q)
+    for b in range(seq_lens.shape[0]):
+        s0, s1 = int(q_start[b]), int(q_start[b + 1])
+        ql, sl = s1 - s0, int(seq_lens[b])
+        if ql <= 0 or sl <= 0:
+            continue
+        blocks = block_tables[b, : (sl + 63) // 64].long()
+        kv = []
+        for cache, gs in ((k_cache, k_scale), (v_cache, v_scale)):
+            codes, scales = _kv_fp4_views(cache[blocks], d)
+            kv.append(kv_fp4_dequantize(codes, scales, gs).permute(1, 0, 2, 3).reshape(hk, -1, d)[:, :sl])
+        k, v = kv
+        qq = q[s0:s1].float().view(ql, hk, hq // hk, d).permute(1, 2, 0, 3)
+        sc = torch.einsum("hgqd,hkd->hgqk", qq, k) * scale
+        mask = torch.arange(sl)[None, :] > torch.arange(sl - ql, sl)[:, None]
+        sc = sc.masked_fill(mask, float("-inf"))
+        p = torch.where(mask.all(-1)[:, None], torch.zeros_like(sc), sc.softmax(-1))
+        out[s0:s1] = torch.einsum("hgqk,hkd->hgqd", p, v).permute(2, 0, 1, 3).reshape(ql, hq, d).to(q.dtype)
+    return out
+
+
 def silu_mul(x: torch.Tensor) -> torch.Tensor:
     f = x.shape[-1] // 2
     xf = x.float()
