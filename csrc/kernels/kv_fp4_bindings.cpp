@@ -194,15 +194,26 @@ void paged_attention_fp4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cac
   p.whole_units = invariant ? 1 : 0;
   p.scale_log2 = static_cast<float>(scale * k_scale * kLog2e);
   p.v_scale = static_cast<float>(v_scale);
-  // Rows of one kv head that a CTA holds: as many as the longest query has, up to what its registers carry.
-  const int64_t rows = std::min<int64_t>(max_q_len, 64) * (hq / hk);
-  const int tile = static_cast<int>(std::min<int64_t>((rows + 7) / 8 * 8, d == 256 ? 16 : 32));
-  const int ctas = sh_paged_attention_fp4_ctas(static_cast<int>(d), tile);
-  TORCH_CHECK(ctas > 0, who, ": no CUDA device");
-  const Scratch s = scratch(k_cache, stream, sh_paged_attention_fp4_workspace(static_cast<int>(d), tile), ctas);
-  p.part_o = s.part.data_ptr<float>();
-  p.tickets = reinterpret_cast<unsigned*>(s.tickets.data_ptr<int>());
-  const int r = sh_paged_attention_fp4(&p, static_cast<int>(d), tile, stream);
+  const int dim = static_cast<int>(d);
+  const int64_t rows = std::min<int64_t>(max_q_len, 4096) * (hq / hk);  // of one kv head
+  int r;
+  if (rows > 32 && d <= 128 && !invariant) {
+    const int tickets = sh_paged_attention_fp4_tc_tickets();
+    TORCH_CHECK(tickets > 0, who, ": no CUDA device");
+    const Scratch s = scratch(k_cache, stream, sh_paged_attention_fp4_tc_workspace(dim), tickets);
+    p.part_o = s.part.data_ptr<float>();
+    p.tickets = reinterpret_cast<unsigned*>(s.tickets.data_ptr<int>());
+    r = sh_paged_attention_fp4_tc(&p, dim, stream);
+  } else {
+    // Rows that a CTA holds: as many as the longest query has, up to what its registers carry.
+    const int tile = static_cast<int>(std::min<int64_t>((rows + 7) / 8 * 8, d == 256 ? 16 : 32));
+    const int ctas = sh_paged_attention_fp4_ctas(dim, tile);
+    TORCH_CHECK(ctas > 0, who, ": no CUDA device");
+    const Scratch s = scratch(k_cache, stream, sh_paged_attention_fp4_workspace(dim, tile), ctas);
+    p.part_o = s.part.data_ptr<float>();
+    p.tickets = reinterpret_cast<unsigned*>(s.tickets.data_ptr<int>());
+    r = sh_paged_attention_fp4(&p, dim, tile, stream);
+  }
   TORCH_CHECK(r == 0, "sh_paged_attention_fp4 failed with code ", r);
 }
 

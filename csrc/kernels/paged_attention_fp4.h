@@ -19,7 +19,7 @@ struct AttnFp4Params {
   const int64_t* seq_lens;       // [B] length including the new tokens
   const int64_t* q_start;        // [B + 1]
   float* part_o;                 // sh_paged_attention_fp4_workspace floats
-  unsigned* tickets;             // one zeroed word per CTA; every call leaves them zero
+  unsigned* tickets;             // zeroed words; every call leaves them zero
   int64_t num_tokens;            // T
   int B, hq, hk, num_blocks, bt_cols;
   int whole_units;               // 1: a (request, head, row tile) is never split over CTAs
@@ -30,12 +30,16 @@ struct AttnFp4Params {
 #ifdef __cplusplus
 extern "C" {
 #endif
-// CTAs of the decode kernel for this head dimension and row tile (also the number of tickets), and the floats of
-// partial results that they may write.  row_tile: query rows of one kv head a CTA holds, 8 * (1..4).
+// CTAs of the kernel for short queries at this head dimension and row tile (also the number of tickets), and the
+// floats of partial results that they may write.  row_tile: query rows of one kv head a CTA holds, 8 * (1..4).
 int sh_paged_attention_fp4_ctas(int head_dim, int row_tile);
 int64_t sh_paged_attention_fp4_workspace(int head_dim, int row_tile);
 // 0 on success; head_dim in {64, 128, 256}, block size 64.
 int sh_paged_attention_fp4(const AttnFp4Params* p, int head_dim, int row_tile, cudaStream_t stream);
+// The tensor-core kernel for many query rows (head_dim 64 or 128): units of 256 rows, whole_units not supported.
+int sh_paged_attention_fp4_tc_tickets(void);
+int64_t sh_paged_attention_fp4_tc_workspace(int head_dim);
+int sh_paged_attention_fp4_tc(const AttnFp4Params* p, int head_dim, cudaStream_t stream);
 #ifdef __cplusplus
 }
 #endif

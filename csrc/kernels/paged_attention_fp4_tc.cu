@@ -1,0 +1,768 @@
+// Paged GQA attention over the 4-bit KV cache on the 5th-generation tensor cores: prompts, chunks of prompts and
+// wide verify windows (paged_attention_fp4.cu states the mathematics and serves short queries).
+//
+// Work.  A unit is (request, kv head, 256 packed query rows): two M = 128 tiles that share every key tile, so a key
+// is decoded once per 256 rows.  The units are laid end to end, each as long as its share of the causal triangle
+// (w_i = ctx G + (i + 1) 256 for tile i: integers with a closed-form sum, so any place is found by bisection), and cut
+// into one run per SM.  A unit cut by a run's end leaves fp32 partials, merged in order by the last of its CTAs.
+//
+// Per CTA (384 threads):
+//   warps 0-3, 4-7   one per query tile, a row a thread (= its TMEM lane): load the row, scale it by a power of two
+//                    into f16's range and store it for the MMA; per key tile read S, softmax in the exp2 domain
+//                    against a reference that moves only when a score passes it by more than 8, write P (f16) over S;
+//                    at the end O / l, or the partial;
+//   warps 8-10       decode 128-key tiles of K and V from the pages into f16 tiles (exact) in shared memory, two
+//                    stages each; the next tile's codes are in registers before a stage is waited for;
+//   warp 11          one thread issues the MMAs: S_q = Q_q K^T, O_q += P_q V, in the order PV_0, S_0', PV_1, S_1', so
+//                    one tile's softmax runs under the other's products.
+// TMEM: S_0, S_1 (128 columns each, P in their first 64), O_0, O_1 (D columns each).
+//
+// Every wait is bounded (2 s); one that runs out raises the CTA's abort flag, the rows of the CTA's units become NaN,
+// and the CTA drains its MMAs and frees its TMEM before it returns.
+#include <float.h>
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "paged_attention_fp4.h"
+#include "pdl.cuh"
+#include "tcgen05_common.cuh"
+
+namespace shk {
+namespace attn4tc {
+
+using namespace shk::tc;
+
+constexpr int PAGE = 64;
+constexpr int KT = 128;    // keys per tile
+constexpr int ROWS = 256;  // query rows per unit
+constexpr int MMA_WARP = 11;
+constexpr int PRODUCERS = 3;
+constexpr int THREADS = 384;  // 12 warps: three to a scheduler, so a thread may hold 168 registers
+constexpr float kSlack = 8.f;
+
+template <int D>
+struct Smem {
+  static constexpr int SLABS = D / 64;            // 64 dimensions: one 128-byte swizzle row
+  static constexpr int SLAB = 128 * 128;          // 128 rows of one slab (queries and keys alike)
+  static constexpr int TILE = SLABS * SLAB;
+  static constexpr int Q = 0;                     // [2]
+  static constexpr int K = Q + 2 * TILE;          // [2]
+  static constexpr int V = K + 2 * TILE;          // [2]
+  static constexpr int BAR = V + 2 * TILE;
+  static constexpr int TOTAL = BAR + 256 + 1024;  // + alignment slack
+};
+
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
+  d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFF) << 32;
+  d |= static_cast<uint64_t>(1) << 46;  // version
+  d |= static_cast<uint64_t>(2) << 61;  // SWIZZLE_128B
+  return d;
+}
+// kind::f16, D f32, A and B f16, A K-major, B K- or MN-major.
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) {
+  return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
+          d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// 32 columns of this thread's lane, without a wait; ld_wait() names the registers, so their uses stay behind it.
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void ld_wait(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t* o) {
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
+      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+      : "r"(w));
+}
+__device__ __forceinline__ uint32_t e4m3x2(uint32_t w) {
+  uint32_t r;
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %1;\n cvt.rn.f16x2.e4m3x2 %0, a;\n}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// What a request asks for, clipped to the tensors it indexes.
+struct Request {
+  int64_t qs, seq, ctx;  // ctx: tokens before the new ones, for the weights (never negative)
+  int q_len, tiles;
+};
+__device__ __forceinline__ Request request(const AttnFp4Params& p, int b) {
+  Request r;
+  const int64_t q0 = p.q_start[b], q1 = p.q_start[b + 1];
+  r.qs = q0 < 0 ? 0 : q0;
+  const int64_t n = (q1 < p.num_tokens ? q1 : p.num_tokens) - r.qs;
+  r.q_len = n > 0 ? static_cast<int>(n) : 0;
+  r.seq = p.seq_lens[b];
+  if (r.seq < 0) r.seq = 0;
+  const int64_t cap = static_cast<int64_t>(p.bt_cols) * PAGE;
+  if (r.seq > cap) r.seq = cap;
+  r.ctx = r.seq > r.q_len ? r.seq - r.q_len : 0;
+  r.tiles = static_cast<int>((static_cast<int64_t>(r.q_len) * (p.hq / p.hk) + ROWS - 1) / ROWS);
+  return r;
+}
+// Cost of the first n row tiles of a request, one kv head.
+__device__ __forceinline__ int64_t cost(const Request& r, int group, int64_t n) {
+  return n * r.ctx * group + ROWS * (n * (n + 1) / 2);
+}
+
+struct Segment {
+  int64_t u0, u1;  // the unit's place among all costs
+  int64_t qs, ctx0, kv_end;
+  int b, h, row0, rows, k0, k1;  // key tiles [k0, k1) of the unit
+  bool whole, head;              // all of the unit; its beginning
+};
+struct Cursor {
+  int64_t pos, end, base;
+  int b;
+  Request r;
+};
+__device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, Segment& s) {
+  if (c.pos >= c.end) return false;
+  const int g = p.hq / p.hk;
+  while (c.pos >= c.base + cost(c.r, g, c.r.tiles) * p.hk) {
+    c.base += cost(c.r, g, c.r.tiles) * p.hk;
+    c.r = request(p, ++c.b);
+  }
+  const int64_t off = c.pos - c.base;
+  int lo = 0, hi = c.r.tiles - 1;  // the tile that holds `off`: its predecessors cost at most that
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cost(c.r, g, mid) * p.hk <= off) lo = mid;
+    else hi = mid - 1;
+  }
+  const int64_t w = c.r.ctx * g + static_cast<int64_t>(lo + 1) * ROWS;
+  const int64_t in = off - cost(c.r, g, lo) * p.hk;
+  s.b = c.b;
+  s.h = static_cast<int>(in / w);
+  s.row0 = lo * ROWS;
+  const int64_t left = static_cast<int64_t>(c.r.q_len) * g - s.row0;
+  s.rows = left < ROWS ? static_cast<int>(left) : ROWS;
+  s.qs = c.r.qs;
+  s.ctx0 = c.r.seq - c.r.q_len;
+  int64_t kv = s.ctx0 + (s.row0 + s.rows - 1) / g + 1;  // keys the tile's last row sees
+  if (kv > c.r.seq) kv = c.r.seq;
+  if (kv < 0) kv = 0;
+  s.kv_end = kv;
+  const int64_t tiles = (kv + KT - 1) / KT;
+  s.u0 = c.pos - in % w;
+  s.u1 = s.u0 + w;
+  const int64_t r0 = c.pos - s.u0, r1 = (c.end < s.u1 ? c.end : s.u1) - s.u0;
+  s.k0 = static_cast<int>(r0 * tiles / w);
+  s.k1 = static_cast<int>(r1 * tiles / w);
+  s.head = r0 == 0;
+  s.whole = s.head && r1 == w;
+  c.pos = s.u0 + r1;
+  return true;
+}
+
+// Eight values, one 16-byte chunk: 8 codes times their block's scale.
+__device__ __forceinline__ uint4 decode8(uint32_t w, uint32_t s2) {
+  uint32_t o[4];
+  e2m1x8(w, o);
+  return make_uint4(hmul2(o[0], s2), hmul2(o[1], s2), hmul2(o[2], s2), hmul2(o[3], s2));
+}
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p) {
+  using M = Smem<D>;
+  constexpr uint32_t T_S = 0, T_O = 2 * KT, T_COLS = 512;
+  constexpr int PAGE_BYTES = PAGE * (D / 2 + D / 16);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + M::BAR);  // each [2]
+  uint64_t* kfull = qfull + 2;
+  uint64_t* kempty = kfull + 2;
+  uint64_t* vfull = kempty + 2;
+  uint64_t* vempty = vfull + 2;
+  uint64_t* sfull = vempty + 2;
+  uint64_t* pfull = sfull + 2;
+  uint64_t* odone = pfull + 2;
+  uint64_t* drain = odone + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* last_flag = abort_flag + 1;  // [2]
+  __shared__ int64_t scan[16];
+  __shared__ int64_t start_base;
+  __shared__ int start_b;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = p.hq / p.hk;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&qfull[i], 4);
+      mbar_init(&kfull[i], PRODUCERS);
+      mbar_init(&kempty[i], 1);
+      mbar_init(&vfull[i], PRODUCERS);
+      mbar_init(&vempty[i], 1);
+      mbar_init(&sfull[i], 1);
+      mbar_init(&pfull[i], 4);
+      mbar_init(&odone[i], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(T_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  shk::pdl_trigger();
+  shk::pdl_wait();  // lengths, tables, queries and the new tokens' rows come from earlier kernels
+
+  // ---------------------------------------------------------------- this CTA's run
+  int64_t total = 0;
+  for (int b = threadIdx.x; b < p.B; b += THREADS) {
+    const Request r = request(p, b);
+    total += cost(r, group, r.tiles) * p.hk;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) scan[warp] = total;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < THREADS / 32; ++w) total += scan[w];
+  __syncthreads();
+  const int64_t per = (total + gridDim.x - 1) / gridDim.x;
+  Cursor cur;
+  cur.pos = per * blockIdx.x;
+  cur.end = cur.pos + per < total ? cur.pos + per : total;
+  if (cur.pos < cur.end) {
+    for (int64_t done = 0, b0 = 0; b0 < p.B; b0 += THREADS) {
+      const int b = static_cast<int>(b0) + threadIdx.x;
+      int64_t w = 0;
+      if (b < p.B) {
+        const Request r = request(p, b);
+        w = cost(r, group, r.tiles) * p.hk;
+      }
+      int64_t incl = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      int64_t before = done;
+      for (int i = 0; i < warp; ++i) before += scan[i];
+      const int64_t hi = before + incl, lo = hi - w;
+      if (lo <= cur.pos && cur.pos < hi) {
+        start_b = b;
+        start_base = lo;
+      }
+      for (int i = 0; i < THREADS / 32; ++i) done += scan[i];
+      __syncthreads();
+      if (done > cur.pos) break;
+    }
+    cur.b = start_b;
+    cur.base = start_base;
+    cur.r = request(p, cur.b);
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Segment s;
+
+  if (warp >= 8 && warp != MMA_WARP) {
+    // ------------------------------------------------------------------ producers
+    // A thread decodes 16-byte pieces (32 dimensions of a key): piece i of a tile is dimensions 32 (i % PR) .. of
+    // key i / PR, so a warp's loads are one run of memory.
+    constexpr int PR = D / 32, PIECES = KT * PR, STEP = PRODUCERS * 32, N = (PIECES + STEP - 1) / STEP;
+    const int tid = threadIdx.x - 256;
+    struct Codes {
+      uint4 w[N];
+      uint32_t sc[N];
+    };
+    auto load = [&](const uint8_t* cache, const Segment& sg, int kt, Codes& c) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int idx = i * STEP + tid, r = idx / PR, d = idx % PR;
+        const int64_t key = static_cast<int64_t>(kt) * KT + r;
+        c.w[i] = make_uint4(0, 0, 0, 0);
+        c.sc[i] = 0;
+        if (idx < PIECES && key < sg.kv_end) {  // a key that no row sees is a zero, whatever its page holds
+          int blk = p.block_tables[static_cast<int64_t>(sg.b) * p.bt_stride + key / PAGE];
+          if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) blk = 0;
+          const uint8_t* pg = cache + (static_cast<int64_t>(blk) * p.hk + sg.h) * PAGE_BYTES;
+          const int tok = static_cast<int>(key % PAGE);
+          c.w[i] = *reinterpret_cast<const uint4*>(pg + tok * (D / 2) + d * 16);
+          c.sc[i] = *reinterpret_cast<const uint16_t*>(pg + PAGE * (D / 2) + tok * (D / 16) + d * 2);
+        }
+      }
+    };
+    auto store = [&](uint8_t* tile, const Codes& c) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int idx = i * STEP + tid, r = idx / PR, d = idx % PR;
+        if (idx >= PIECES) break;
+        const uint32_t pr = e4m3x2(c.sc[i]);
+        const uint32_t s0 = __byte_perm(pr, 0, 0x1010), s1 = __byte_perm(pr, 0, 0x3232);
+        uint8_t* row = tile + (d >> 1) * M::SLAB + r * 128;
+        const int ch = (d & 1) * 4;
+        *reinterpret_cast<uint4*>(row + (((ch + 0) ^ (r & 7)) << 4)) = decode8(c.w[i].x, s0);
+        *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = decode8(c.w[i].y, s0);
+        *reinterpret_cast<uint4*>(row + (((ch + 2) ^ (r & 7)) << 4)) = decode8(c.w[i].z, s1);
+        *reinterpret_cast<uint4*>(row + (((ch + 3) ^ (r & 7)) << 4)) = decode8(c.w[i].w, s1);
+      }
+      fence_proxy_async_smem();  // the decoded tile is read by the tensor cores
+      __syncwarp();
+    };
+    int kc = 0;  // tiles filled so far (K and V alike)
+    bool ok = true;
+    Codes kk, vv;  // while one is decoded, the other's loads are under way
+    bool more = false;
+    do {
+      more = next_segment(p, cur, s);
+    } while (more && s.k0 == s.k1);
+    int kt = s.k0;
+    if (more) load(p.k_cache, s, kt, kk);
+    while (more) {
+      const int st = kc & 1;
+      load(p.v_cache, s, kt, vv);
+      if (kc >= 2 && !__all_sync(0xffffffffu, mbar_wait(&kempty[st], ((kc >> 1) - 1) & 1, abort_flag))) {
+        ok = false;
+        break;
+      }
+      store(smem + M::K + st * M::TILE, kk);
+      if (lane == 0) mbar_arrive(&kfull[st]);
+      if (++kt == s.k1) {
+        do {
+          more = next_segment(p, cur, s);
+        } while (more && s.k0 == s.k1);
+        kt = s.k0;
+      }
+      if (more) load(p.k_cache, s, kt, kk);
+      if (kc >= 2 && !__all_sync(0xffffffffu, mbar_wait(&vempty[st], ((kc >> 1) - 1) & 1, abort_flag))) {
+        ok = false;
+        break;
+      }
+      store(smem + M::V + st * M::TILE, vv);
+      if (lane == 0) mbar_arrive(&vfull[st]);
+      ++kc;
+    }
+    if (!ok) *abort_flag = 1;
+  } else if (warp == MMA_WARP) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t IS = idesc_f16(128, KT, false), IP = idesc_f16(128, D, true);
+      const uint64_t qd = sw128_desc(smem_addr(smem + M::Q)), kd = sw128_desc(smem_addr(smem + M::K));
+      const uint64_t vd = sw128_mn_desc(smem_addr(smem + M::V), M::SLAB, 1024);
+      int kc = 0, nq_done[2] = {0, 0}, np_done[2] = {0, 0};
+      bool ok = true;
+      auto qk = [&](int q, int st) {
+        const uint64_t a = qd + static_cast<uint64_t>((q * M::TILE) >> 4), b = kd + static_cast<uint64_t>((st * M::TILE) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t o = static_cast<uint64_t>(((kk >> 2) * M::SLAB + (kk & 3) * 32) >> 4);
+          mma_ss(tmem + T_S + q * KT, a + o, b + o, IS, kk ? 1u : 0u);
+        }
+        mma_commit(&sfull[q]);
+      };
+      while (ok && next_segment(p, cur, s)) {
+        const int nq = s.rows > 128 ? 2 : 1;
+        if (s.k0 == s.k1) continue;
+        for (int kt = s.k0 - 1; ok && kt < s.k1; ++kt) {
+          // O_q += P_q V of tile kt, then S_q of tile kt + 1 (the first pass has only the latter)
+          const int vst = (kc - 1) & 1, st = kc & 1;
+          const bool pv = kt >= s.k0, next = kt + 1 < s.k1;
+          if (pv) ok = mbar_wait(&vfull[vst], ((kc - 1) >> 1) & 1, abort_flag);
+          for (int q = 0; ok && q < nq; ++q) {
+            if (pv) {
+              ok = mbar_wait(&pfull[q], np_done[q]++ & 1, abort_flag);
+              if (!ok) break;
+              fence_after();
+              const uint64_t b = vd + static_cast<uint64_t>((vst * M::TILE) >> 4);
+#pragma unroll
+              for (int kk = 0; kk < KT / 16; ++kk)
+                mma_ts(tmem + T_O + q * D, tmem + T_S + q * KT + kk * 8, b + static_cast<uint64_t>((kk * 2048) >> 4), IP,
+                       (kt > s.k0 || kk > 0) ? 1u : 0u);
+              if (!next) mma_commit(&odone[q]);
+            } else {
+              ok = mbar_wait(&qfull[q], nq_done[q]++ & 1, abort_flag);
+              if (!ok) break;
+            }
+            if (next) {
+              if (q == 0) ok = mbar_wait(&kfull[st], (kc >> 1) & 1, abort_flag);
+              if (!ok) break;
+              fence_after();
+              qk(q, st);
+            }
+          }
+          if (ok && pv) mma_commit(&vempty[vst]);
+          if (ok && next) {
+            mma_commit(&kempty[st]);
+            ++kc;
+          }
+        }
+      }
+      if (!ok) *abort_flag = 1;
+      mma_commit(drain);
+      (void)mbar_wait_drain(drain, 0);
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax + epilogue
+    const int q = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t tl = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + tl + T_S + q * KT, tO = tmem + tl + T_O + q * D;
+    int ns = 0, no = 0;  // S tiles and finished units seen so far
+    bool ok = true;
+    while (next_segment(p, cur, s)) {
+      if (q * 128 >= s.rows) continue;
+      const int n = q * 128 + r;
+      const bool valid = n < s.rows;
+      const int rr = s.row0 + n;
+      const int64_t tok = s.qs + rr / group;
+      const int head = s.h * group + rr % group;
+      const int64_t pos = s.ctx0 + rr / group;
+      float m = -FLT_MAX, l = 0.f, cs = 0.f;
+      if (s.k0 < s.k1 && ok) {
+        // the query row, its largest element scaled into [2^13, 2^14)
+        uint32_t top = 0;
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + tok * p.q_stride + static_cast<int64_t>(head) * D);
+        uint4 raw[D / 8];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          raw[i] = valid ? src[i] : make_uint4(0, 0, 0, 0);
+          const uint32_t w4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, max(w4[k] & 0x7fffu, (w4[k] >> 16) & 0x7fffu));
+        }
+        const int e = min(267 - static_cast<int>(top >> 7), 253);
+        const float f = __uint_as_float(static_cast<uint32_t>(e) << 23);
+        cs = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * p.scale_log2;
+        uint8_t* qrow = smem + M::Q + q * M::TILE + r * 128;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t w4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          uint32_t o[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            o[k] = pack_f16(__uint_as_float(w4[k] << 16) * f, __uint_as_float(w4[k] & 0xffff0000u) * f);
+          *reinterpret_cast<uint4*>(qrow + (i >> 3) * M::SLAB + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&qfull[q]);
+
+        const int64_t safe = s.ctx0 + (s.row0 + q * 128) / group;  // the tile's first position
+        for (int kt = s.k0; kt < s.k1; ++kt, ++ns) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&sfull[q], ns & 1, abort_flag))) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          const int64_t key0 = static_cast<int64_t>(kt) * KT;
+          const bool edge = key0 + KT - 1 > safe;
+          // keys [0, lim) of the tile are this row's
+          const int lim = edge ? static_cast<int>(min(max(pos + 1 - key0, int64_t(0)), int64_t(KT))) : KT;
+          float sum = 0.f;
+          uint32_t buf[2][32];
+          ld32(tS, buf[0]);
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c) {
+            uint32_t* x = buf[c & 1];
+            ld_wait(x);
+            if (c + 1 < KT / 32) ld32(tS + 32 * (c + 1), buf[(c + 1) & 1]);
+            // distances from the reference, masked keys at -infinity
+            auto shift = [&]() {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                float v = fmaf(__uint_as_float(x[i]), cs, -m);
+                if (edge && c * 32 + i >= lim) v = -INFINITY;
+                x[i] = __float_as_uint(v);
+              }
+            };
+            shift();
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
+            if (__any_sync(0xffffffffu, mx > kSlack)) {
+              // rare: the scores again (P has not reached their columns yet), and their maximum
+              if (c + 1 < KT / 32) ld_wait(buf[(c + 1) & 1]);
+              st_wait();
+              ld32(tS + 32 * c, x);
+              ld_wait(x);
+              float hi = -FLT_MAX;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(edge && c * 32 + i >= lim)) hi = fmaxf(hi, __uint_as_float(x[i]) * cs);
+              const float to = mx > kSlack ? hi : m;
+              const float al = ex2(m - to);
+              l *= al;
+              sum *= al;
+              m = to;
+              shift();
+              // what this tile has written of P, and O (which holds every earlier tile: S of this one was issued
+              // behind their products)
+#pragma unroll 1
+              for (int i = 0; i < c; ++i) {
+                uint32_t pk[32];  // chunk i of P is the first 16 of these columns
+                ld32(tS + 16 * i, pk);
+                ld_wait(pk);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&pk[k]));
+                  pk[k] = pack_f16(v.x * al, v.y * al);
+                }
+                st16(tS + 16 * i, pk);
+                st_wait();
+              }
+              if (kt > s.k0) {
+#pragma unroll 1
+                for (int i = 0; i < D; i += 32) {
+                  uint32_t o[32];
+                  ld32(tO + i, o);
+                  ld_wait(o);
+#pragma unroll
+                  for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * al);
+                  st32(tO + i, o);
+                }
+                st_wait();
+              }
+            }
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float p0 = ex2(__uint_as_float(x[2 * i])), p1 = ex2(__uint_as_float(x[2 * i + 1]));
+              sum += p0 + p1;
+              pk[i] = pack_f16(p0, p1);
+            }
+            st16(tS + 16 * c, pk);
+          }
+          l += sum;
+          st_wait();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pfull[q]);
+        }
+        if (ok && !__all_sync(0xffffffffu, mbar_wait(&odone[q], no & 1, abort_flag))) ok = false;
+        ++no;
+        if (!ok) *abort_flag = 1;
+        fence_after();
+      }
+      if (!ok) l = __uint_as_float(0x7fc00000u);  // a wait ran out: NaN, not numbers
+      const bool none = s.k0 == s.k1 || !ok;
+      const int cta = blockIdx.x;
+      auto part = [&](int c, bool head_slot) {
+        return p.part_o + (static_cast<int64_t>(2 * c + (head_slot ? 1 : 0)) * 2 + q) * (D + 2) * 128 + r;
+      };
+      if (s.whole) {
+        const float inv = l == 0.f ? 0.f : p.v_scale / l;  // no key at all: 0 (a NaN stays one)
+        __nv_bfloat16* dst = p.out + tok * p.out_stride + static_cast<int64_t>(head) * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          if (none) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = 0;
+          } else {
+            ld32(tO + c, o);
+            ld_wait(o);
+          }
+          if (valid) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t v[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                v[i] = pack_bf16(__uint_as_float(o[8 * k + 2 * i]) * inv, __uint_as_float(o[8 * k + 2 * i + 1]) * inv);
+              *reinterpret_cast<uint4*>(dst + c + 8 * k) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+        continue;
+      }
+      float* mine = part(cta, s.head);
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (none) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = 0;
+        } else {
+          ld32(tO + c, o);
+          ld_wait(o);
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) mine[(c + k) * 128] = __uint_as_float(o[k]);
+      }
+      mine[D * 128] = m;
+      mine[(D + 1) * 128] = l;
+      __threadfence();
+      named_barrier(1 + q, 128);
+      const int first = static_cast<int>(s.u0 / per), last = static_cast<int>((s.u1 - 1) / per);
+      if (r == 0) {
+        unsigned* ticket = p.tickets + 2 * first + q;
+        const bool is_last = atomicAdd(ticket, 1u) == static_cast<unsigned>(last - first);
+        last_flag[q] = is_last;
+        if (is_last) *ticket = 0;
+        __threadfence();
+      }
+      named_barrier(1 + q, 128);
+      if (last_flag[q]) {
+        float top = -FLT_MAX, den = 0.f;
+        for (int c = first; c <= last; ++c) top = fmaxf(top, __ldcg(part(c, c == first) + D * 128));
+        for (int c = first; c <= last; ++c)
+          den += ex2(__ldcg(part(c, c == first) + D * 128) - top) * __ldcg(part(c, c == first) + (D + 1) * 128);
+        const float inv = den == 0.f ? 0.f : p.v_scale / den;
+        __nv_bfloat16* dst = p.out + tok * p.out_stride + static_cast<int64_t>(head) * D;
+#pragma unroll 1
+        for (int d = 0; d < D; d += 16) {
+          float acc[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) acc[k] = 0.f;
+          for (int c = first; c <= last; ++c) {
+            const float* src = part(c, c == first);
+            const float wt = ex2(__ldcg(src + D * 128) - top);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[k] += wt * __ldcg(src + (d + k) * 128);
+          }
+          if (valid) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              *reinterpret_cast<uint4*>(dst + d + 8 * k) =
+                  make_uint4(pack_bf16(acc[8 * k] * inv, acc[8 * k + 1] * inv), pack_bf16(acc[8 * k + 2] * inv, acc[8 * k + 3] * inv),
+                             pack_bf16(acc[8 * k + 4] * inv, acc[8 * k + 5] * inv), pack_bf16(acc[8 * k + 6] * inv, acc[8 * k + 7] * inv));
+          }
+        }
+      }
+      named_barrier(1 + q, 128);  // last_flag is rewritten by the next unit
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(T_COLS));
+  }
+}
+
+}  // namespace attn4tc
+}  // namespace shk
+
+using namespace shk::attn4tc;
+
+namespace {
+constexpr int kMaxDevices = 64;
+
+int num_sms() {
+  static int sms[kMaxDevices] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  if (!sms[dev] && cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return sms[dev];
+}
+
+template <int D>
+int launch(const AttnFp4Params& p, cudaStream_t st) {
+  static_assert(Smem<D>::TOTAL + 256 <= 227 * 1024, "shared-memory budget");
+  static bool ready[kMaxDevices] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -5;
+  auto k = attn_fp4_tc_kernel<D>;
+  if (!ready[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL);
+    if (e != cudaSuccess) return 300 + static_cast<int>(e);
+    ready[dev] = true;
+  }
+  const int ctas = num_sms();
+  if (ctas <= 0) return -5;
+  const cudaError_t e = shk::launch(k, dim3(ctas), dim3(THREADS), Smem<D>::TOTAL, st, p);
+  return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
+}
+}  // namespace
+
+extern "C" int sh_paged_attention_fp4_tc_tickets(void) { return 2 * num_sms(); }
+
+extern "C" int64_t sh_paged_attention_fp4_tc_workspace(int head_dim) {
+  return static_cast<int64_t>(num_sms()) * 4 * (head_dim + 2) * 128;
+}
+
+extern "C" int sh_paged_attention_fp4_tc(const AttnFp4Params* params, int head_dim, cudaStream_t stream) {
+  const AttnFp4Params& p = *params;
+  if (p.num_tokens <= 0 || p.B <= 0) return 0;
+  if (p.hk <= 0 || p.hq % p.hk != 0 || p.num_blocks <= 0 || p.bt_cols <= 0 || p.whole_units) return -1;
+  if (p.part_o == nullptr || p.tickets == nullptr) return -2;
+  if ((reinterpret_cast<uintptr_t>(p.k_cache) & 15) || (reinterpret_cast<uintptr_t>(p.v_cache) & 15) ||
+      (reinterpret_cast<uintptr_t>(p.q) & 15) || (p.q_stride & 7) || (reinterpret_cast<uintptr_t>(p.out) & 15) ||
+      (p.out_stride & 7))
+    return -3;
+  switch (head_dim) {
+    case 64: return launch<64>(p, stream);
+    case 128: return launch<128>(p, stream);
+    default: return -4;
+  }
+}

@@ -77,7 +77,7 @@ def oracle(c):
             p = torch.softmax(torch.where(seen[:, None], sc, -math.inf), -1)
             p = torch.where(seen.any(1)[:, None, None], p, 0.0)
             out[s0:s1, hs] = p @ v
-            size = torch.einsum("tgd,nd->tgn", c["q"][s0:s1].view(-1, hq, d)[:, hs].double().abs(), k.abs()) * c["scale"]
+            size = torch.einsum("tgd,nd->tgn", c["q"][s0:s1].view(-1, hq, d)[:, hs].double().abs(), k.abs()) * abs(c["scale"])
             score = 2 * (d / 16 + 2) * 2.0 ** -23 * torch.where(seen[:, None], size, 0.0).amax(-1, keepdim=True)
             tol[s0:s1, hs] = (2.0 ** -11 + 2.0 ** -18 + score) * (p @ v.abs()) + n * 2.0 ** -25 * v.abs().max()
     return out, tol + 2.0 ** -8 * out.abs() + 1e-9
@@ -118,6 +118,43 @@ def test_verify_window_ragged(hq, hk, d):
 @pytest.mark.parametrize("q,seqs", [((200,), (200,)), ((65, 130, 1), (65, 400, 90)), ((33, 257), (1000, 257))])
 def test_prefill_and_chunks(hq, hk, d, q, seqs):
     c = case(q, seqs, hq, hk, d, seed=5)
+    check(c, attend(c))
+
+
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (4, 4, 64), (7, 1, 128), (40, 1, 64), (12, 2, 128)])
+@pytest.mark.parametrize("q,seqs", [((33,), (33,)), ((64, 17), (9000, 129)), ((129, 257, 1, 0, 63), (129, 300, 5000, 40, 64)),
+                                    ((700,), (1500,))])
+def test_many_rows(hq, hk, d, q, seqs):
+    """Row tiles of one to many rows, one or both halves of a unit, units split over several CTAs and many in one."""
+    c = case(q, seqs, hq, hk, d, seed=20 + d)
+    check(c, attend(c))
+
+
+def test_many_rows_that_see_nothing():
+    c = case((90, 70, 40), (30, 0, 40), 8, 2, 128, seed=21)
+    got = attend(c)
+    check(c, got)
+    assert (got[:60] == 0).all() and (got[90:160] == 0).all() and (got[60:90] != 0).any(1).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_many_rows_with_a_rising_maximum(d):
+    """Keys that grow along the sequence: the softmax reference moves in almost every tile, inside tiles too."""
+    c = case((150,), (1500,), 4, 2, d, seed=22)
+    x = torch.randn(c["k"].shape[0], 2, 64, d, generator=torch.Generator().manual_seed(22))
+    n = c["bt"].shape[1]
+    x[c["bt"][0].long()] *= (torch.arange(n * 64).view(n, 1, 64, 1) / 100.0).exp2().clamp(max=400.0)
+    codes, scales = ops.ref.kv_fp4_quantize(x)
+    c["k"] = torch.cat((codes.flatten(2), scales.flatten(2)), 2).contiguous()
+    c["q"] *= torch.logspace(-20, 3, 150, base=2.0)[:, None].bfloat16()
+    check(c, attend(c))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125])
+@pytest.mark.parametrize("q", [1, 100])
+def test_zero_and_negative_scale(scale, q):
+    c = case((q,), (300,), 8, 2, 128, seed=23)
+    c["scale"] = scale
     check(c, attend(c))
 
 
