@@ -3,7 +3,8 @@
 //
 // Work.  A unit is (request, kv head, 256 packed query rows): two M = 128 tiles that share every key tile, so a key
 // is decoded once per 256 rows.  The units are laid end to end, each as long as its share of the causal triangle
-// (w_i = ctx G + (i + 1) 256 for tile i: integers with a closed-form sum, so any place is found by bisection), and cut
+// (w_i = (ctx + c) G + (i + 1) 256 for tile i, c for its start and end: integers with a closed-form sum, so any place
+// is found by bisection), and cut
 // into one run per SM.  A unit cut by a run's end leaves fp32 partials, merged in order by the last of its CTAs.
 //
 // Per CTA (384 threads):
@@ -42,6 +43,7 @@ constexpr int MMA_WARP = 11;
 constexpr int PRODUCERS = 3;
 constexpr int THREADS = 384;  // 12 warps: three to a scheduler, so a thread may hold 168 registers
 constexpr float kSlack = 8.f;
+constexpr int kUnit = 256;  // a unit's start and end in keys
 
 template <int D>
 struct Smem {
@@ -101,15 +103,19 @@ __device__ __forceinline__ void ld_wait(uint32_t* r) {
                :
                : "memory");
 }
-__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
+__device__ __forceinline__ void ld8(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -153,6 +159,39 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+
 // What a request asks for, clipped to the tensors it indexes.
 struct Request {
   int64_t qs, seq, ctx;  // ctx: tokens before the new ones, for the weights (never negative)
@@ -172,9 +211,13 @@ __device__ __forceinline__ Request request(const AttnFp4Params& p, int b) {
   r.tiles = static_cast<int>((static_cast<int64_t>(r.q_len) * (p.hq / p.hk) + ROWS - 1) / ROWS);
   return r;
 }
-// Cost of the first n row tiles of a request, one kv head.
+// Cost of a request's row tile i, one kv head: the keys it sees (times the group) and kUnit keys for what a unit costs
+// besides; and of its first n tiles.
+__device__ __forceinline__ int64_t tile_cost(const Request& r, int group, int64_t i) {
+  return (r.ctx + kUnit) * group + (i + 1) * ROWS;
+}
 __device__ __forceinline__ int64_t cost(const Request& r, int group, int64_t n) {
-  return n * r.ctx * group + ROWS * (n * (n + 1) / 2);
+  return n * (r.ctx + kUnit) * group + ROWS * (n * (n + 1) / 2);
 }
 
 struct Segment {
@@ -202,7 +245,7 @@ __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, 
     if (cost(c.r, g, mid) * p.hk <= off) lo = mid;
     else hi = mid - 1;
   }
-  const int64_t w = c.r.ctx * g + static_cast<int64_t>(lo + 1) * ROWS;
+  const int64_t w = tile_cost(c.r, g, lo);
   const int64_t in = off - cost(c.r, g, lo) * p.hk;
   s.b = c.b;
   s.h = static_cast<int>(in / w);
@@ -257,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
   __shared__ int64_t start_base;
   __shared__ int start_b;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int group = p.hq / p.hk;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -346,132 +389,165 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
       uint4 w[N];
       uint32_t sc[N];
     };
-    auto load = [&](const uint8_t* cache, const Segment& sg, int kt, Codes& c) {
+    // a page's pieces lie one behind the other: piece idx of the tile is piece idx % (PIECES / 2) of its page
+    auto load = [&](const uint8_t* cache, const Segment& sg, int kt) {
+      Codes c;
+      const uint8_t* pg[KT / PAGE];
+#pragma unroll
+      for (int i = 0; i < KT / PAGE; ++i) {
+        const int64_t page = static_cast<int64_t>(kt) * (KT / PAGE) + i;
+        int blk = page * PAGE < sg.kv_end ? p.block_tables[static_cast<int64_t>(sg.b) * p.bt_stride + page] : 0;
+        if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) blk = 0;
+        pg[i] = cache + (static_cast<int64_t>(blk) * p.hk + sg.h) * PAGE_BYTES;
+      }
+      const int64_t left = sg.kv_end - static_cast<int64_t>(kt) * KT;
+      const int live = left < KT ? static_cast<int>(left) * PR : PIECES;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int idx = i * STEP + tid, r = idx / PR, d = idx % PR;
-        const int64_t key = static_cast<int64_t>(kt) * KT + r;
+        const int idx = i * STEP + tid;
         c.w[i] = make_uint4(0, 0, 0, 0);
         c.sc[i] = 0;
-        if (idx < PIECES && key < sg.kv_end) {  // a key that no row sees is a zero, whatever its page holds
-          int blk = p.block_tables[static_cast<int64_t>(sg.b) * p.bt_stride + key / PAGE];
-          if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) blk = 0;
-          const uint8_t* pg = cache + (static_cast<int64_t>(blk) * p.hk + sg.h) * PAGE_BYTES;
-          const int tok = static_cast<int>(key % PAGE);
-          c.w[i] = *reinterpret_cast<const uint4*>(pg + tok * (D / 2) + d * 16);
-          c.sc[i] = *reinterpret_cast<const uint16_t*>(pg + PAGE * (D / 2) + tok * (D / 16) + d * 2);
+        if (idx < live) {  // a key that no row sees is a zero, whatever its page holds
+          const uint8_t* base = idx < PIECES / 2 ? pg[0] : pg[1];
+          const int in = idx & (PIECES / 2 - 1);
+          c.w[i] = *reinterpret_cast<const uint4*>(base + in * 16);
+          c.sc[i] = *reinterpret_cast<const uint16_t*>(base + PAGE * (D / 2) + in * 2);
         }
       }
+      return c;
     };
+    // A thread's pieces are all the same 32 dimensions.  The threads of the second 64 write their four chunks in the
+    // order 2, 3, 0, 1: in step with the first 64's they would meet in the same banks.
+    const int d = tid % PR;
+    const bool turned = D > 64 && (d & 2);
+    const int ch = (d & 1) * 4, c0 = turned ? 2 : 0;
     auto store = [&](uint8_t* tile, const Codes& c) {
+      uint8_t* slab = tile + (d >> 1) * M::SLAB;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int idx = i * STEP + tid, r = idx / PR, d = idx % PR;
+        const int idx = i * STEP + tid, r = idx / PR;
         if (idx >= PIECES) break;
         const uint32_t pr = e4m3x2(c.sc[i]);
-        const uint32_t s0 = __byte_perm(pr, 0, 0x1010), s1 = __byte_perm(pr, 0, 0x3232);
-        uint8_t* row = tile + (d >> 1) * M::SLAB + r * 128;
-        const int ch = (d & 1) * 4;
-        *reinterpret_cast<uint4*>(row + (((ch + 0) ^ (r & 7)) << 4)) = decode8(c.w[i].x, s0);
-        *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = decode8(c.w[i].y, s0);
-        *reinterpret_cast<uint4*>(row + (((ch + 2) ^ (r & 7)) << 4)) = decode8(c.w[i].z, s1);
-        *reinterpret_cast<uint4*>(row + (((ch + 3) ^ (r & 7)) << 4)) = decode8(c.w[i].w, s1);
+        const uint32_t sa = __byte_perm(pr, 0, turned ? 0x3232 : 0x1010), sb = __byte_perm(pr, 0, turned ? 0x1010 : 0x3232);
+        const uint32_t a0 = turned ? c.w[i].z : c.w[i].x, a1 = turned ? c.w[i].w : c.w[i].y;
+        const uint32_t b0 = turned ? c.w[i].x : c.w[i].z, b1 = turned ? c.w[i].y : c.w[i].w;
+        uint8_t* row = slab + r * 128;
+        const int at = (ch + c0) ^ (r & 7);  // chunk positions differ from it in their low two bits
+        *reinterpret_cast<uint4*>(row + (at << 4)) = decode8(a0, sa);
+        *reinterpret_cast<uint4*>(row + ((at ^ 1) << 4)) = decode8(a1, sa);
+        *reinterpret_cast<uint4*>(row + ((at ^ 2) << 4)) = decode8(b0, sb);
+        *reinterpret_cast<uint4*>(row + ((at ^ 3) << 4)) = decode8(b1, sb);
       }
       fence_proxy_async_smem();  // the decoded tile is read by the tensor cores
       __syncwarp();
     };
-    int kc = 0;  // tiles filled so far (K and V alike)
-    bool ok = true;
-    Codes kk, vv;  // while one is decoded, the other's loads are under way
-    bool more = false;
-    do {
-      more = next_segment(p, cur, s);
-    } while (more && s.k0 == s.k1);
+    // Items in the order K(0), V(0), K(1), ...: item n fills stage (n / 2) % 2 of its ring.  While one is decoded the
+    // next one's loads are under way.
+    auto settle = [&]() {  // the next unit with keys
+      bool more;
+      do {
+        more = next_segment(p, cur, s);
+      } while (more && s.k0 == s.k1);
+      return more;
+    };
+    bool ok = true, more = settle();
     int kt = s.k0;
-    if (more) load(p.k_cache, s, kt, kk);
-    while (more) {
-      const int st = kc & 1;
-      load(p.v_cache, s, kt, vv);
-      if (kc >= 2 && !__all_sync(0xffffffffu, mbar_wait(&kempty[st], ((kc >> 1) - 1) & 1, abort_flag))) {
-        ok = false;
-        break;
-      }
-      store(smem + M::K + st * M::TILE, kk);
-      if (lane == 0) mbar_arrive(&kfull[st]);
-      if (++kt == s.k1) {
-        do {
-          more = next_segment(p, cur, s);
-        } while (more && s.k0 == s.k1);
+    Codes now;
+    if (more) now = load(p.k_cache, s, kt);
+#pragma unroll 1
+    for (int n = 0; more; ++n) {
+      const int v = n & 1, st = (n >> 1) & 1, turn = n >> 2;
+      if (v && ++kt == s.k1) {
+        more = settle();
         kt = s.k0;
       }
-      if (more) load(p.k_cache, s, kt, kk);
-      if (kc >= 2 && !__all_sync(0xffffffffu, mbar_wait(&vempty[st], ((kc >> 1) - 1) & 1, abort_flag))) {
+      Codes next;
+      if (more) next = load(v ? p.k_cache : p.v_cache, s, kt);
+      uint64_t* empty = (v ? vempty : kempty) + st;
+      if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(empty, (turn - 1) & 1, abort_flag))) {
         ok = false;
         break;
       }
-      store(smem + M::V + st * M::TILE, vv);
-      if (lane == 0) mbar_arrive(&vfull[st]);
-      ++kc;
+      store(smem + (v ? M::V : M::K) + st * M::TILE, now);
+      if (lane == 0) mbar_arrive((v ? vfull : kfull) + st);
+      now = next;
     }
     if (!ok) *abort_flag = 1;
   } else if (warp == MMA_WARP) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t IS = idesc_f16(128, KT, false), IP = idesc_f16(128, D, true);
-      const uint64_t qd = sw128_desc(smem_addr(smem + M::Q)), kd = sw128_desc(smem_addr(smem + M::K));
-      const uint64_t vd = sw128_mn_desc(smem_addr(smem + M::V), M::SLAB, 1024);
-      int kc = 0, nq_done[2] = {0, 0}, np_done[2] = {0, 0};
-      bool ok = true;
-      auto qk = [&](int q, int st) {
-        const uint64_t a = qd + static_cast<uint64_t>((q * M::TILE) >> 4), b = kd + static_cast<uint64_t>((st * M::TILE) >> 4);
+    // The whole warp walks the loop, on values that the compiler can see to be uniform, and one elected lane (the same
+    // each time) issues: operands then stay in uniform registers, where a lone lane's would be moved there for every
+    // MMA.  The election stands at each use: with its result kept in a variable this compiler's code gave wrong sums.
+    constexpr uint32_t IS = idesc_f16(128, KT, false), IP = idesc_f16(128, D, true);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t sbase = __shfl_sync(0xffffffffu, smem_addr(smem), 0);
+    const uint64_t qd = sw128_desc(sbase + M::Q), kd = sw128_desc(sbase + M::K);
+    const uint64_t vd = sw128_mn_desc(sbase + M::V, M::SLAB, 1024);
+    int kc = 0, np[2] = {0, 0}, nqf[2] = {0, 0};  // key tiles, P tiles and queries consumed so far
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
+    while (ok) {
+      const bool more = next_segment(p, cur, s);
+      if (!__shfl_sync(0xffffffffu, static_cast<int>(more), 0)) break;
+      const int nq = __shfl_sync(0xffffffffu, s.rows, 0) > 128 ? 2 : 1;
+      const int tiles = __shfl_sync(0xffffffffu, s.k1 - s.k0, 0);
+      if (tiles == 0) continue;
+      for (int j = -1; ok && j < tiles; ++j) {
+        // O_q += P_q V of tile j, then S_q of tile j + 1 (the first pass has only the latter)
+        const int vst = (kc - 1) & 1, st = kc & 1;
+        const bool pv = j >= 0, next = j + 1 < tiles;
+        if (pv) ok = wait(&vfull[vst], ((kc - 1) >> 1) & 1);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t o = static_cast<uint64_t>(((kk >> 2) * M::SLAB + (kk & 3) * 32) >> 4);
-          mma_ss(tmem + T_S + q * KT, a + o, b + o, IS, kk ? 1u : 0u);
-        }
-        mma_commit(&sfull[q]);
-      };
-      while (ok && next_segment(p, cur, s)) {
-        const int nq = s.rows > 128 ? 2 : 1;
-        if (s.k0 == s.k1) continue;
-        for (int kt = s.k0 - 1; ok && kt < s.k1; ++kt) {
-          // O_q += P_q V of tile kt, then S_q of tile kt + 1 (the first pass has only the latter)
-          const int vst = (kc - 1) & 1, st = kc & 1;
-          const bool pv = kt >= s.k0, next = kt + 1 < s.k1;
-          if (pv) ok = mbar_wait(&vfull[vst], ((kc - 1) >> 1) & 1, abort_flag);
-          for (int q = 0; ok && q < nq; ++q) {
-            if (pv) {
-              ok = mbar_wait(&pfull[q], np_done[q]++ & 1, abort_flag);
-              if (!ok) break;
-              fence_after();
+        for (int q = 0; q < 2; ++q) {
+          if (q >= nq || !ok) break;
+          if (pv) {
+            ok = wait(&pfull[q], np[q] & 1);
+            ++np[q];
+            if (!ok) break;
+            fence_after();
+            if (elect_one()) {
               const uint64_t b = vd + static_cast<uint64_t>((vst * M::TILE) >> 4);
 #pragma unroll
               for (int kk = 0; kk < KT / 16; ++kk)
-                mma_ts(tmem + T_O + q * D, tmem + T_S + q * KT + kk * 8, b + static_cast<uint64_t>((kk * 2048) >> 4), IP,
-                       (kt > s.k0 || kk > 0) ? 1u : 0u);
+                mma_ts(tm + T_O + q * D, tm + T_S + q * KT + kk * 8, b + static_cast<uint64_t>((kk * 2048) >> 4), IP,
+                       (j > 0 || kk > 0) ? 1u : 0u);
               if (!next) mma_commit(&odone[q]);
-            } else {
-              ok = mbar_wait(&qfull[q], nq_done[q]++ & 1, abort_flag);
-              if (!ok) break;
             }
-            if (next) {
-              if (q == 0) ok = mbar_wait(&kfull[st], (kc >> 1) & 1, abort_flag);
-              if (!ok) break;
-              fence_after();
-              qk(q, st);
+          } else {
+            ok = wait(&qfull[q], nqf[q] & 1);
+            ++nqf[q];
+            if (!ok) break;
+          }
+          if (next) {
+            if (q == 0) ok = wait(&kfull[st], (kc >> 1) & 1);
+            if (!ok) break;
+            fence_after();
+            if (elect_one()) {
+              const uint64_t a = qd + static_cast<uint64_t>((q * M::TILE) >> 4);
+              const uint64_t b = kd + static_cast<uint64_t>((st * M::TILE) >> 4);
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk) {
+                const uint64_t o = static_cast<uint64_t>(((kk >> 2) * M::SLAB + (kk & 3) * 32) >> 4);
+                mma_ss(tm + T_S + q * KT, a + o, b + o, IS, kk ? 1u : 0u);
+              }
+              mma_commit(&sfull[q]);
             }
           }
-          if (ok && pv) mma_commit(&vempty[vst]);
-          if (ok && next) {
-            mma_commit(&kempty[st]);
-            ++kc;
-          }
+          __syncwarp();
         }
+        if (ok && elect_one()) {
+          if (pv) mma_commit(&vempty[vst]);
+          if (next) mma_commit(&kempty[st]);
+        }
+        if (next) ++kc;
       }
-      if (!ok) *abort_flag = 1;
+    }
+    if (!ok) *abort_flag = 1;
+    if (elect_one()) {
       mma_commit(drain);
       (void)mbar_wait_drain(drain, 0);
     }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------------ softmax + epilogue
     const int q = warp >> 2, r = threadIdx.x & 127;
@@ -501,8 +577,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
           for (int k = 0; k < 4; ++k) top = max(top, max(w4[k] & 0x7fffu, (w4[k] >> 16) & 0x7fffu));
         }
         const int e = min(267 - static_cast<int>(top >> 7), 253);
-        const float f = __uint_as_float(static_cast<uint32_t>(e) << 23);
-        cs = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * p.scale_log2;
+        // the scale's sign goes with the row (0: a zero row), so that cs > 0 and the largest S is the largest score
+        const float f = p.scale_log2 == 0.f ? 0.f : copysignf(__uint_as_float(static_cast<uint32_t>(e) << 23), p.scale_log2);
+        cs = fmaxf(__uint_as_float(static_cast<uint32_t>(254 - e) << 23) * fabsf(p.scale_log2), FLT_MIN);
         uint8_t* qrow = smem + M::Q + q * M::TILE + r * 128;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
@@ -528,81 +605,81 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
           const bool edge = key0 + KT - 1 > safe;
           // keys [0, lim) of the tile are this row's
           const int lim = edge ? static_cast<int>(min(max(pos + 1 - key0, int64_t(0)), int64_t(KT))) : KT;
-          float sum = 0.f;
-          uint32_t buf[2][32];
-          ld32(tS, buf[0]);
-#pragma unroll
-          for (int c = 0; c < KT / 32; ++c) {
-            uint32_t* x = buf[c & 1];
+          uint64_t sum[2] = {0, 0};
+          // two halves of 64 columns, one copy of the code: the roles share one instruction cache
+#pragma unroll 1
+          for (int c = 0; c < KT; c += 64) {
+            uint32_t x[64];
+            ld32(tS + c, x);
+            ld32(tS + c + 32, x + 32);
             ld_wait(x);
-            if (c + 1 < KT / 32) ld32(tS + 32 * (c + 1), buf[(c + 1) & 1]);
-            // distances from the reference, masked keys at -infinity
-            auto shift = [&]() {
+            ld_wait(x + 32);
+            if (edge) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                float v = fmaf(__uint_as_float(x[i]), cs, -m);
-                if (edge && c * 32 + i >= lim) v = -INFINITY;
-                x[i] = __float_as_uint(v);
-              }
-            };
-            shift();
-            float mx = -INFINITY;
+              for (int i = 0; i < 64; ++i)
+                if (c + i >= lim) x[i] = __float_as_uint(-INFINITY);
+            }
+            const float* f = reinterpret_cast<const float*>(x);
+            float t4[4];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
-            if (__any_sync(0xffffffffu, mx > kSlack)) {
-              // rare: the scores again (P has not reached their columns yet), and their maximum
-              if (c + 1 < KT / 32) ld_wait(buf[(c + 1) & 1]);
-              st_wait();
-              ld32(tS + 32 * c, x);
-              ld_wait(x);
-              float hi = -FLT_MAX;
+            for (int i = 0; i < 4; ++i) t4[i] = max3(f[i], f[4 + i], f[8 + i]);
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(edge && c * 32 + i >= lim)) hi = fmaxf(hi, __uint_as_float(x[i]) * cs);
-              const float to = mx > kSlack ? hi : m;
+            for (int j = 12; j < 60; j += 8)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) t4[i] = max3(t4[i], f[j + i], f[j + 4 + i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t4[i] = fmaxf(t4[i], f[60 + i]);
+            const float mx = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]);
+            const bool grow = fmaf(mx, cs, -m) > kSlack;
+            if (__any_sync(0xffffffffu, grow)) {  // rare
+              const float to = grow ? mx * cs : m;
               const float al = ex2(m - to);
-              l *= al;
-              sum *= al;
               m = to;
-              shift();
+              l *= al;
+              sum[0] = fma2(sum[0], pair(al, al), 0);
+              sum[1] = fma2(sum[1], pair(al, al), 0);
               // what this tile has written of P, and O (which holds every earlier tile: S of this one was issued
               // behind their products)
+              st_wait();
 #pragma unroll 1
-              for (int i = 0; i < c; ++i) {
-                uint32_t pk[32];  // chunk i of P is the first 16 of these columns
-                ld32(tS + 16 * i, pk);
-                ld_wait(pk);
+              for (int i = 0; i < c / 2; i += 8) {
+                uint32_t pk[8];
+                ld8(tS + i, pk);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
+                for (int k = 0; k < 8; ++k) {
                   const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&pk[k]));
                   pk[k] = pack_f16(v.x * al, v.y * al);
                 }
-                st16(tS + 16 * i, pk);
-                st_wait();
+                st8(tS + i, pk);
               }
-              if (kt > s.k0) {
 #pragma unroll 1
-                for (int i = 0; i < D; i += 32) {
-                  uint32_t o[32];
-                  ld32(tO + i, o);
-                  ld_wait(o);
+              for (int i = 0; i < (kt > s.k0 ? D : 0); i += 8) {
+                uint32_t o[8];
+                ld8(tO + i, o);
 #pragma unroll
-                  for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * al);
-                  st32(tO + i, o);
-                }
-                st_wait();
+                for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * al);
+                st8(tO + i, o);
               }
+              st_wait();
             }
-            uint32_t pk[16];
+            const uint64_t cs2 = pair(cs, cs), nm2 = pair(-m, -m);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float p0 = ex2(__uint_as_float(x[2 * i])), p1 = ex2(__uint_as_float(x[2 * i + 1]));
-              sum += p0 + p1;
-              pk[i] = pack_f16(p0, p1);
+            for (int h = 0; h < 64; h += 32) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 v = unpair(fma2(pair(f[h + 2 * i], f[h + 2 * i + 1]), cs2, nm2));
+                const float p0 = ex2(v.x), p1 = ex2(v.y);
+                sum[i & 1] = add2(sum[i & 1], pair(p0, p1));
+                pk[i] = pack_f16(p0, p1);
+              }
+              st16(tS + (c + h) / 2, pk);
             }
-            st16(tS + 16 * c, pk);
           }
-          l += sum;
+          {
+            const float2 a = unpair(sum[0]), b = unpair(sum[1]);
+            l += (a.x + a.y) + (b.x + b.y);
+          }
           st_wait();
           fence_before();
           __syncwarp();
