@@ -197,7 +197,7 @@ void paged_attention_fp4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cac
   const int dim = static_cast<int>(d);
   const int64_t rows = std::min<int64_t>(max_q_len, 4096) * (hq / hk);  // of one kv head
   int r;
-  if (rows > 32 && d <= 128 && !invariant) {
+  if (rows > 32 && !invariant) {
     const int tickets = sh_paged_attention_fp4_tc_tickets();
     TORCH_CHECK(tickets > 0, who, ": no CUDA device");
     const Scratch s = scratch(k_cache, stream, sh_paged_attention_fp4_tc_workspace(dim), tickets);

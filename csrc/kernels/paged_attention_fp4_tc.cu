@@ -1,22 +1,23 @@
 // Paged GQA attention over the 4-bit KV cache on the 5th-generation tensor cores: prompts, chunks of prompts and
 // wide verify windows (paged_attention_fp4.cu states the mathematics and serves short queries).
 //
-// Work.  A unit is (request, kv head, 256 packed query rows): two M = 128 tiles that share every key tile, so a key
-// is decoded once per 256 rows.  The units are laid end to end, each as long as its share of the causal triangle
-// (w_i = (ctx + c) G + (i + 1) 256 for tile i, c for its start and end: integers with a closed-form sum, so any place
-// is found by bisection), and cut
-// into one run per SM.  A unit cut by a run's end leaves fp32 partials, merged in order by the last of its CTAs.
+// Work.  A unit is (request, kv head, NQ tiles of 128 packed query rows) that share every key tile, so a key is decoded
+// once per 256 rows (128 at head_dim 256, where two accumulators do not fit TMEM).  The units are laid end to end,
+// each as long as its share of the causal triangle (w_i = (ctx + c) G + (i + 1) ROWS for row tile i, c for a unit's
+// start and end: integers with a closed-form sum, so any place is found by bisection), and cut into one run per SM.  A
+// unit cut by a run's end leaves fp32 partials, merged in order by the last of its CTAs.
 //
-// Per CTA (384 threads):
-//   warps 0-3, 4-7   one per query tile, a row a thread (= its TMEM lane): load the row, scale it by a power of two
-//                    into f16's range and store it for the MMA; per key tile read S, softmax in the exp2 domain
+// Per CTA (512 threads):
+//   warps 0-3, 4-7   one warpgroup per query tile, a row a thread (= its TMEM lane): load the row, scale it by a power
+//                    of two into f16's range and store it for the MMA; per key tile read S, softmax in the exp2 domain
 //                    against a reference that moves only when a score passes it by more than 8, write P (f16) over S;
 //                    at the end O / l, or the partial;
-//   warps 8-10       decode 128-key tiles of K and V from the pages into f16 tiles (exact) in shared memory, two
-//                    stages each; the next tile's codes are in registers before a stage is waited for;
-//   warp 11          one thread issues the MMAs: S_q = Q_q K^T, O_q += P_q V, in the order PV_0, S_0', PV_1, S_1', so
-//                    one tile's softmax runs under the other's products.
-// TMEM: S_0, S_1 (128 columns each, P in their first 64), O_0, O_1 (D columns each).
+//   warps 8-10, 11-13 decode 64-key tiles (a page's head) of K and of V into f16 tiles (exact) in shared memory; the
+//                    next two tiles' codes are on their way in registers;
+//   warps 14, 15     issue the MMAs of a query tile each: S_q = Q_q K^T into one of two buffers, O_q += P_q V.  S of the next tile is
+//                    issued before P of this one is waited for, so the softmax never waits for a product it could have
+//                    had, and the products run under the other tile's (or buffer's) softmax.
+// TMEM: S_q,b (64 columns each, P in their first 32), O_q (D columns each) from column 256.
 //
 // Every wait is bounded (2 s); one that runs out raises the CTA's abort flag, the rows of the CTA's units become NaN,
 // and the CTA drains its MMAs and frees its TMEM before it returns.
@@ -37,24 +38,28 @@ namespace attn4tc {
 using namespace shk::tc;
 
 constexpr int PAGE = 64;
-constexpr int KT = 128;    // keys per tile
-constexpr int ROWS = 256;  // query rows per unit
-constexpr int MMA_WARP = 11;
-constexpr int PRODUCERS = 3;
-constexpr int THREADS = 384;  // 12 warps: three to a scheduler, so a thread may hold 168 registers
+constexpr int KT = PAGE;  // keys per tile
+constexpr int PRODUCERS = 3;  // warps each for K and V
+constexpr int MMA_WARP = 8 + 2 * PRODUCERS;
+constexpr int THREADS = (MMA_WARP + 2) * 32;
 constexpr float kSlack = 8.f;
 constexpr int kUnit = 256;  // a unit's start and end in keys
 
 template <int D>
 struct Smem {
+  static constexpr int NQ = D == 256 ? 1 : 2;     // query tiles
+  static constexpr int ROWS = 128 * NQ;           // query rows per unit
+  static constexpr int STAGES = D == 256 ? 2 : 4;
   static constexpr int SLABS = D / 64;            // 64 dimensions: one 128-byte swizzle row
-  static constexpr int SLAB = 128 * 128;          // 128 rows of one slab (queries and keys alike)
-  static constexpr int TILE = SLABS * SLAB;
-  static constexpr int Q = 0;                     // [2]
-  static constexpr int K = Q + 2 * TILE;          // [2]
-  static constexpr int V = K + 2 * TILE;          // [2]
-  static constexpr int BAR = V + 2 * TILE;
-  static constexpr int TOTAL = BAR + 256 + 1024;  // + alignment slack
+  static constexpr int QSLAB = 128 * 128;         // 128 rows of one slab
+  static constexpr int KSLAB = KT * 128;
+  static constexpr int QTILE = SLABS * QSLAB;
+  static constexpr int KTILE = SLABS * KSLAB;
+  static constexpr int Q = 0;                     // [NQ]
+  static constexpr int K = Q + NQ * QTILE;        // [STAGES]
+  static constexpr int V = K + STAGES * KTILE;    // [STAGES]
+  static constexpr int BAR = V + STAGES * KTILE;
+  static constexpr int TOTAL = BAR + 512 + 1024;  // + alignment slack
 };
 
 __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
@@ -197,6 +202,7 @@ struct Request {
   int64_t qs, seq, ctx;  // ctx: tokens before the new ones, for the weights (never negative)
   int q_len, tiles;
 };
+template <int ROWS>
 __device__ __forceinline__ Request request(const AttnFp4Params& p, int b) {
   Request r;
   const int64_t q0 = p.q_start[b], q1 = p.q_start[b + 1];
@@ -213,9 +219,11 @@ __device__ __forceinline__ Request request(const AttnFp4Params& p, int b) {
 }
 // Cost of a request's row tile i, one kv head: the keys it sees (times the group) and kUnit keys for what a unit costs
 // besides; and of its first n tiles.
+template <int ROWS>
 __device__ __forceinline__ int64_t tile_cost(const Request& r, int group, int64_t i) {
   return (r.ctx + kUnit) * group + (i + 1) * ROWS;
 }
+template <int ROWS>
 __device__ __forceinline__ int64_t cost(const Request& r, int group, int64_t n) {
   return n * (r.ctx + kUnit) * group + ROWS * (n * (n + 1) / 2);
 }
@@ -231,22 +239,23 @@ struct Cursor {
   int b;
   Request r;
 };
+template <int ROWS>
 __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, Segment& s) {
   if (c.pos >= c.end) return false;
   const int g = p.hq / p.hk;
-  while (c.pos >= c.base + cost(c.r, g, c.r.tiles) * p.hk) {
-    c.base += cost(c.r, g, c.r.tiles) * p.hk;
-    c.r = request(p, ++c.b);
+  while (c.pos >= c.base + cost<ROWS>(c.r, g, c.r.tiles) * p.hk) {
+    c.base += cost<ROWS>(c.r, g, c.r.tiles) * p.hk;
+    c.r = request<ROWS>(p, ++c.b);
   }
   const int64_t off = c.pos - c.base;
   int lo = 0, hi = c.r.tiles - 1;  // the tile that holds `off`: its predecessors cost at most that
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (cost(c.r, g, mid) * p.hk <= off) lo = mid;
+    if (cost<ROWS>(c.r, g, mid) * p.hk <= off) lo = mid;
     else hi = mid - 1;
   }
-  const int64_t w = tile_cost(c.r, g, lo);
-  const int64_t in = off - cost(c.r, g, lo) * p.hk;
+  const int64_t w = tile_cost<ROWS>(c.r, g, lo);
+  const int64_t in = off - cost<ROWS>(c.r, g, lo) * p.hk;
   s.b = c.b;
   s.h = static_cast<int>(in / w);
   s.row0 = lo * ROWS;
@@ -280,20 +289,21 @@ __device__ __forceinline__ uint4 decode8(uint32_t w, uint32_t s2) {
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p) {
   using M = Smem<D>;
-  constexpr uint32_t T_S = 0, T_O = 2 * KT, T_COLS = 512;
+  constexpr int ROWS = M::ROWS, NQ = M::NQ, STAGES = M::STAGES;
+  constexpr uint32_t T_S = 0, T_O = 256, T_COLS = 512;
   constexpr int PAGE_BYTES = PAGE * (D / 2 + D / 16);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + M::BAR);  // each [2]
-  uint64_t* kfull = qfull + 2;
-  uint64_t* kempty = kfull + 2;
-  uint64_t* vfull = kempty + 2;
-  uint64_t* vempty = vfull + 2;
-  uint64_t* sfull = vempty + 2;
-  uint64_t* pfull = sfull + 2;
-  uint64_t* odone = pfull + 2;
-  uint64_t* drain = odone + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + M::BAR);  // [2]
+  uint64_t* kfull = qfull + 2;                                   // [STAGES], as the next three
+  uint64_t* kempty = kfull + STAGES;
+  uint64_t* vfull = kempty + STAGES;
+  uint64_t* vempty = vfull + STAGES;
+  uint64_t* sfull = vempty + STAGES;                             // [q][buffer]
+  uint64_t* pfull = sfull + 4;                                   // [q][buffer]
+  uint64_t* pvdone = pfull + 4;                                  // [q][buffer]: the product of that P is in O
+  uint64_t* drain = pvdone + 4;                                  // [q]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* last_flag = abort_flag + 1;  // [2]
   __shared__ int64_t scan[16];
@@ -305,15 +315,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&qfull[i], 4);
+      mbar_init(&drain[i], 1);
+    }
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(&kfull[i], PRODUCERS);
-      mbar_init(&kempty[i], 1);
+      mbar_init(&kempty[i], NQ);
       mbar_init(&vfull[i], PRODUCERS);
-      mbar_init(&vempty[i], 1);
+      mbar_init(&vempty[i], NQ);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&sfull[i], 1);
       mbar_init(&pfull[i], 4);
-      mbar_init(&odone[i], 1);
+      mbar_init(&pvdone[i], 1);
     }
-    mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -328,8 +342,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
   // ---------------------------------------------------------------- this CTA's run
   int64_t total = 0;
   for (int b = threadIdx.x; b < p.B; b += THREADS) {
-    const Request r = request(p, b);
-    total += cost(r, group, r.tiles) * p.hk;
+    const Request r = request<ROWS>(p, b);
+    total += cost<ROWS>(r, group, r.tiles) * p.hk;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -347,8 +361,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
       const int b = static_cast<int>(b0) + threadIdx.x;
       int64_t w = 0;
       if (b < p.B) {
-        const Request r = request(p, b);
-        w = cost(r, group, r.tiles) * p.hk;
+        const Request r = request<ROWS>(p, b);
+        w = cost<ROWS>(r, group, r.tiles) * p.hk;
       }
       int64_t incl = w;
 #pragma unroll
@@ -371,58 +385,74 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
     }
     cur.b = start_b;
     cur.base = start_base;
-    cur.r = request(p, cur.b);
+    cur.r = request<ROWS>(p, cur.b);
   }
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
-  Segment s;
+  Segment s = {};
 
-  if (warp >= 8 && warp != MMA_WARP) {
+  if (warp >= 8 && warp < MMA_WARP) {
     // ------------------------------------------------------------------ producers
     // A thread decodes 16-byte pieces (32 dimensions of a key): piece i of a tile is dimensions 32 (i % PR) .. of
     // key i / PR, so a warp's loads are one run of memory.
     constexpr int PR = D / 32, PIECES = KT * PR, STEP = PRODUCERS * 32, N = (PIECES + STEP - 1) / STEP;
-    const int tid = threadIdx.x - 256;
+    const bool value = warp >= 8 + PRODUCERS;  // this warp's matrix
+    const int tid = threadIdx.x - (value ? 8 + PRODUCERS : 8) * 32;
+    const uint8_t* cache = value ? p.v_cache : p.k_cache;
     struct Codes {
       uint4 w[N];
       uint32_t sc[N];
     };
-    // a page's pieces lie one behind the other: piece idx of the tile is piece idx % (PIECES / 2) of its page
-    auto load = [&](const uint8_t* cache, const Segment& sg, int kt) {
-      Codes c;
-      const uint8_t* pg[KT / PAGE];
-#pragma unroll
-      for (int i = 0; i < KT / PAGE; ++i) {
-        const int64_t page = static_cast<int64_t>(kt) * (KT / PAGE) + i;
-        int blk = page * PAGE < sg.kv_end ? p.block_tables[static_cast<int64_t>(sg.b) * p.bt_stride + page] : 0;
-        if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) blk = 0;
-        pg[i] = cache + (static_cast<int64_t>(blk) * p.hk + sg.h) * PAGE_BYTES;
+    bool more;
+    int asked = 0;  // tiles asked for so far
+    int kt, blk, nxt;  // the tile whose codes are asked for next, its block and the following tile's
+    auto block_of = [&](int tile) {
+      int b = static_cast<int64_t>(tile) * KT < s.kv_end ? p.block_tables[static_cast<int64_t>(s.b) * p.bt_stride + tile] : 0;
+      return static_cast<unsigned>(b) < static_cast<unsigned>(p.num_blocks) ? b : 0;
+    };
+    auto settle = [&]() {  // the next unit with keys
+      do {
+        more = next_segment<ROWS>(p, cur, s);
+      } while (more && s.k0 == s.k1);
+      kt = s.k0;
+      if (more) {
+        blk = block_of(kt);
+        nxt = block_of(kt + 1);
       }
-      const int64_t left = sg.kv_end - static_cast<int64_t>(kt) * KT;
+    };
+    auto fetch = [&]() {  // the next tile's codes, wherever its unit
+      Codes c = {};
+      if (!more) return c;
+      ++asked;
+      const uint8_t* pg = cache + (static_cast<int64_t>(blk) * p.hk + s.h) * PAGE_BYTES;
+      const int64_t left = s.kv_end - static_cast<int64_t>(kt) * KT;
       const int live = left < KT ? static_cast<int>(left) * PR : PIECES;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int idx = i * STEP + tid;
-        c.w[i] = make_uint4(0, 0, 0, 0);
-        c.sc[i] = 0;
         if (idx < live) {  // a key that no row sees is a zero, whatever its page holds
-          const uint8_t* base = idx < PIECES / 2 ? pg[0] : pg[1];
-          const int in = idx & (PIECES / 2 - 1);
-          c.w[i] = *reinterpret_cast<const uint4*>(base + in * 16);
-          c.sc[i] = *reinterpret_cast<const uint16_t*>(base + PAGE * (D / 2) + in * 2);
+          c.w[i] = *reinterpret_cast<const uint4*>(pg + idx * 16);
+          c.sc[i] = *reinterpret_cast<const uint16_t*>(pg + PAGE * (D / 2) + idx * 2);
         }
+      }
+      if (++kt == s.k1) {
+        settle();
+      } else {
+        blk = nxt;
+        nxt = block_of(kt + 1);
       }
       return c;
     };
     // A thread's pieces are all the same 32 dimensions.  The threads of the second 64 write their four chunks in the
     // order 2, 3, 0, 1: in step with the first 64's they would meet in the same banks.
+    static_assert(STEP % PR == 0, "a thread keeps its dimensions");
     const int d = tid % PR;
     const bool turned = D > 64 && (d & 2);
-    const int ch = (d & 1) * 4, c0 = turned ? 2 : 0;
+    const int ch = (d & 1) * 4 + (turned ? 2 : 0);
     auto store = [&](uint8_t* tile, const Codes& c) {
-      uint8_t* slab = tile + (d >> 1) * M::SLAB;
+      uint8_t* slab = tile + (d >> 1) * M::KSLAB;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int idx = i * STEP + tid, r = idx / PR;
@@ -432,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
         const uint32_t a0 = turned ? c.w[i].z : c.w[i].x, a1 = turned ? c.w[i].w : c.w[i].y;
         const uint32_t b0 = turned ? c.w[i].x : c.w[i].z, b1 = turned ? c.w[i].y : c.w[i].w;
         uint8_t* row = slab + r * 128;
-        const int at = (ch + c0) ^ (r & 7);  // chunk positions differ from it in their low two bits
+        const int at = ch ^ (r & 7);  // chunk positions differ from it in their low two bits
         *reinterpret_cast<uint4*>(row + (at << 4)) = decode8(a0, sa);
         *reinterpret_cast<uint4*>(row + ((at ^ 1) << 4)) = decode8(a1, sa);
         *reinterpret_cast<uint4*>(row + ((at ^ 2) << 4)) = decode8(b0, sb);
@@ -441,121 +471,109 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
       fence_proxy_async_smem();  // the decoded tile is read by the tensor cores
       __syncwarp();
     };
-    // Items in the order K(0), V(0), K(1), ...: item n fills stage (n / 2) % 2 of its ring.  While one is decoded the
-    // next one's loads are under way.
-    auto settle = [&]() {  // the next unit with keys
-      bool more;
-      do {
-        more = next_segment(p, cur, s);
-      } while (more && s.k0 == s.k1);
-      return more;
-    };
-    bool ok = true, more = settle();
-    int kt = s.k0;
-    Codes now;
-    if (more) now = load(p.k_cache, s, kt);
+    uint64_t* full = value ? vfull : kfull;
+    uint64_t* empty = value ? vempty : kempty;
+    bool ok = true;
+    settle();
+    Codes now = fetch(), then = fetch();
 #pragma unroll 1
-    for (int n = 0; more; ++n) {
-      const int v = n & 1, st = (n >> 1) & 1, turn = n >> 2;
-      if (v && ++kt == s.k1) {
-        more = settle();
-        kt = s.k0;
-      }
-      Codes next;
-      if (more) next = load(v ? p.k_cache : p.v_cache, s, kt);
-      uint64_t* empty = (v ? vempty : kempty) + st;
-      if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(empty, (turn - 1) & 1, abort_flag))) {
+    for (int n = 0; n < asked; ++n) {  // tile n fills stage n % STAGES
+      const int st = n % STAGES, turn = n / STAGES;
+      if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(empty + st, (turn - 1) & 1, abort_flag))) {
         ok = false;
         break;
       }
-      store(smem + (v ? M::V : M::K) + st * M::TILE, now);
-      if (lane == 0) mbar_arrive((v ? vfull : kfull) + st);
-      now = next;
+      store(smem + (value ? M::V : M::K) + st * M::KTILE, now);
+      if (lane == 0) mbar_arrive(full + st);
+      now = then;
+      then = fetch();
     }
     if (!ok) *abort_flag = 1;
-  } else if (warp == MMA_WARP) {
+  } else if (warp >= MMA_WARP && warp < MMA_WARP + NQ) {
     // ------------------------------------------------------------------ MMA issuer
     // The whole warp walks the loop, on values that the compiler can see to be uniform, and one elected lane (the same
     // each time) issues: operands then stay in uniform registers, where a lone lane's would be moved there for every
-    // MMA.  The election stands at each use: with its result kept in a variable this compiler's code gave wrong sums.
+    // MMA (about 125 cycles an MMA instead of 25).
     constexpr uint32_t IS = idesc_f16(128, KT, false), IP = idesc_f16(128, D, true);
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t sbase = __shfl_sync(0xffffffffu, smem_addr(smem), 0);
-    const uint64_t qd = sw128_desc(sbase + M::Q), kd = sw128_desc(sbase + M::K);
-    const uint64_t vd = sw128_mn_desc(sbase + M::V, M::SLAB, 1024);
-    int kc = 0, np[2] = {0, 0}, nqf[2] = {0, 0};  // key tiles, P tiles and queries consumed so far
+    const uint64_t kd = sw128_desc(sbase + M::K);
+    const uint64_t vd = sw128_mn_desc(sbase + M::V, M::KSLAB, 1024);
+    const int q = warp - MMA_WARP;
+    const uint64_t qd = sw128_desc(sbase + M::Q + q * M::QTILE);
+    const uint32_t ts = tm + T_S + q * 2 * KT, to = tm + T_O + q * D;
+    int kc = 0, vc = 0, qc = 0, sc = 0, pc = 0;  // K and V tiles, queries, S and P so far
     bool ok = true;
     auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
     while (ok) {
-      const bool more = next_segment(p, cur, s);
+      const bool more = next_segment<ROWS>(p, cur, s);
       if (!__shfl_sync(0xffffffffu, static_cast<int>(more), 0)) break;
-      const int nq = __shfl_sync(0xffffffffu, s.rows, 0) > 128 ? 2 : 1;
+      const bool mine = __shfl_sync(0xffffffffu, s.rows, 0) > q * 128;  // this tile has rows
       const int tiles = __shfl_sync(0xffffffffu, s.k1 - s.k0, 0);
-      if (tiles == 0) continue;
+      if (tiles > 0 && mine) {
+        ok = wait(&qfull[q], qc & 1);
+        ++qc;
+      }
+#pragma unroll 1
       for (int j = -1; ok && j < tiles; ++j) {
-        // O_q += P_q V of tile j, then S_q of tile j + 1 (the first pass has only the latter)
-        const int vst = (kc - 1) & 1, st = kc & 1;
-        const bool pv = j >= 0, next = j + 1 < tiles;
-        if (pv) ok = wait(&vfull[vst], ((kc - 1) >> 1) & 1);
+        if (j + 1 < tiles) {  // S of tile j + 1
+          const int st = kc % STAGES;
+          ok = wait(&kfull[st], (kc / STAGES) & 1);
+          if (!ok) break;
+          ++kc;
+          fence_after();
+          if (elect_one()) {
+            if (mine) {
+              const uint64_t b = kd + static_cast<uint64_t>((st * M::KTILE) >> 4);
+              const uint32_t d = ts + (sc & 1) * KT;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          if (q >= nq || !ok) break;
-          if (pv) {
-            ok = wait(&pfull[q], np[q] & 1);
-            ++np[q];
-            if (!ok) break;
-            fence_after();
-            if (elect_one()) {
-              const uint64_t b = vd + static_cast<uint64_t>((vst * M::TILE) >> 4);
-#pragma unroll
-              for (int kk = 0; kk < KT / 16; ++kk)
-                mma_ts(tm + T_O + q * D, tm + T_S + q * KT + kk * 8, b + static_cast<uint64_t>((kk * 2048) >> 4), IP,
-                       (j > 0 || kk > 0) ? 1u : 0u);
-              if (!next) mma_commit(&odone[q]);
+              for (int kk = 0; kk < D / 16; ++kk)
+                mma_ss(d, qd + static_cast<uint64_t>(((kk >> 2) * M::QSLAB + (kk & 3) * 32) >> 4),
+                       b + static_cast<uint64_t>(((kk >> 2) * M::KSLAB + (kk & 3) * 32) >> 4), IS, kk ? 1u : 0u);
+              mma_commit(&sfull[q * 2 + (sc & 1)]);
             }
-          } else {
-            ok = wait(&qfull[q], nqf[q] & 1);
-            ++nqf[q];
-            if (!ok) break;
-          }
-          if (next) {
-            if (q == 0) ok = wait(&kfull[st], (kc >> 1) & 1);
-            if (!ok) break;
-            fence_after();
-            if (elect_one()) {
-              const uint64_t a = qd + static_cast<uint64_t>((q * M::TILE) >> 4);
-              const uint64_t b = kd + static_cast<uint64_t>((st * M::TILE) >> 4);
-#pragma unroll
-              for (int kk = 0; kk < D / 16; ++kk) {
-                const uint64_t o = static_cast<uint64_t>(((kk >> 2) * M::SLAB + (kk & 3) * 32) >> 4);
-                mma_ss(tm + T_S + q * KT, a + o, b + o, IS, kk ? 1u : 0u);
-              }
-              mma_commit(&sfull[q]);
-            }
+            mma_commit(&kempty[st]);
           }
           __syncwarp();
+          sc += mine ? 1 : 0;
         }
-        if (ok && elect_one()) {
-          if (pv) mma_commit(&vempty[vst]);
-          if (next) mma_commit(&kempty[st]);
+        if (j >= 0) {  // O += P V of tile j
+          const int st = vc % STAGES, buf = pc & 1;
+          ok = wait(&vfull[st], (vc / STAGES) & 1) && (!mine || wait(&pfull[q * 2 + buf], (pc >> 1) & 1));
+          if (!ok) break;
+          ++vc;
+          fence_after();
+          if (elect_one()) {
+            if (mine) {
+              const uint64_t b = vd + static_cast<uint64_t>((st * M::KTILE) >> 4);
+#pragma unroll
+              for (int kk = 0; kk < KT / 16; ++kk)
+                mma_ts(to, ts + buf * KT + kk * 8, b + static_cast<uint64_t>((kk * 2048) >> 4), IP, (j > 0 || kk > 0) ? 1u : 0u);
+              mma_commit(&pvdone[q * 2 + buf]);
+            }
+            mma_commit(&vempty[st]);
+          }
+          __syncwarp();
+          pc += mine ? 1 : 0;
         }
-        if (next) ++kc;
       }
     }
     if (!ok) *abort_flag = 1;
     if (elect_one()) {
-      mma_commit(drain);
-      (void)mbar_wait_drain(drain, 0);
+      mma_commit(&drain[q]);
+      (void)mbar_wait_drain(&drain[q], 0);
     }
     __syncwarp();
-  } else {
+  } else if (warp < 4 * NQ) {
     // ------------------------------------------------------------------ softmax + epilogue
     const int q = warp >> 2, r = threadIdx.x & 127;
     const uint32_t tl = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + tl + T_S + q * KT, tO = tmem + tl + T_O + q * D;
-    int ns = 0, no = 0;  // S tiles and finished units seen so far
+    const uint32_t tO = tmem + tl + T_O + q * D;
+    // S tiles seen so far.  A barrier belongs to one buffer: its next phase cannot complete before this warp has been
+    // through the last, so a parity is never two phases old.
+    int ns = 0;
     bool ok = true;
-    while (next_segment(p, cur, s)) {
+    while (next_segment<ROWS>(p, cur, s)) {
       if (q * 128 >= s.rows) continue;
       const int n = q * 128 + r;
       const bool valid = n < s.rows;
@@ -580,7 +598,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
         // the scale's sign goes with the row (0: a zero row), so that cs > 0 and the largest S is the largest score
         const float f = p.scale_log2 == 0.f ? 0.f : copysignf(__uint_as_float(static_cast<uint32_t>(e) << 23), p.scale_log2);
         cs = fmaxf(__uint_as_float(static_cast<uint32_t>(254 - e) << 23) * fabsf(p.scale_log2), FLT_MIN);
-        uint8_t* qrow = smem + M::Q + q * M::TILE + r * 128;
+        uint8_t* qrow = smem + M::Q + q * M::QTILE + r * 128;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           const uint32_t w4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -588,7 +606,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             o[k] = pack_f16(__uint_as_float(w4[k] << 16) * f, __uint_as_float(w4[k] & 0xffff0000u) * f);
-          *reinterpret_cast<uint4*>(qrow + (i >> 3) * M::SLAB + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(qrow + (i >> 3) * M::QSLAB + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -596,7 +614,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
 
         const int64_t safe = s.ctx0 + (s.row0 + q * 128) / group;  // the tile's first position
         for (int kt = s.k0; kt < s.k1; ++kt, ++ns) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&sfull[q], ns & 1, abort_flag))) {
+          const int buf = q * 2 + (ns & 1);
+          const uint32_t tS = tmem + tl + T_S + buf * KT;
+          if (!__all_sync(0xffffffffu, mbar_wait(&sfull[buf], (ns >> 1) & 1, abort_flag))) {
             ok = false;
             break;
           }
@@ -606,54 +626,41 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
           // keys [0, lim) of the tile are this row's
           const int lim = edge ? static_cast<int>(min(max(pos + 1 - key0, int64_t(0)), int64_t(KT))) : KT;
           uint64_t sum[2] = {0, 0};
-          // two halves of 64 columns, one copy of the code: the roles share one instruction cache
-#pragma unroll 1
-          for (int c = 0; c < KT; c += 64) {
-            uint32_t x[64];
-            ld32(tS + c, x);
-            ld32(tS + c + 32, x + 32);
-            ld_wait(x);
-            ld_wait(x + 32);
-            if (edge) {
+          uint32_t x[64];
+          ld32(tS, x);
+          ld32(tS + 32, x + 32);
+          ld_wait(x);
+          ld_wait(x + 32);
+          if (edge) {
 #pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (c + i >= lim) x[i] = __float_as_uint(-INFINITY);
-            }
-            const float* f = reinterpret_cast<const float*>(x);
-            float t4[4];
+            for (int i = 0; i < 64; ++i)
+              if (i >= lim) x[i] = __float_as_uint(-INFINITY);
+          }
+          const float* f = reinterpret_cast<const float*>(x);
+          float t4[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t4[i] = max3(f[i], f[4 + i], f[8 + i]);
+          for (int i = 0; i < 4; ++i) t4[i] = max3(f[i], f[4 + i], f[8 + i]);
 #pragma unroll
-            for (int j = 12; j < 60; j += 8)
+          for (int j = 12; j < 60; j += 8)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) t4[i] = max3(t4[i], f[j + i], f[j + 4 + i]);
+            for (int i = 0; i < 4; ++i) t4[i] = max3(t4[i], f[j + i], f[j + 4 + i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t4[i] = fmaxf(t4[i], f[60 + i]);
-            const float mx = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]);
-            const bool grow = fmaf(mx, cs, -m) > kSlack;
-            if (__any_sync(0xffffffffu, grow)) {  // rare
-              const float to = grow ? mx * cs : m;
-              const float al = ex2(m - to);
-              m = to;
-              l *= al;
-              sum[0] = fma2(sum[0], pair(al, al), 0);
-              sum[1] = fma2(sum[1], pair(al, al), 0);
-              // what this tile has written of P, and O (which holds every earlier tile: S of this one was issued
-              // behind their products)
-              st_wait();
-#pragma unroll 1
-              for (int i = 0; i < c / 2; i += 8) {
-                uint32_t pk[8];
-                ld8(tS + i, pk);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&pk[k]));
-                  pk[k] = pack_f16(v.x * al, v.y * al);
-                }
-                st8(tS + i, pk);
+          for (int i = 0; i < 4; ++i) t4[i] = fmaxf(t4[i], f[60 + i]);
+          const float mx = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]);
+          const bool grow = fmaf(mx, cs, -m) > kSlack;
+          if (__any_sync(0xffffffffu, grow)) {  // rare
+            const float to = grow ? mx * cs : m;
+            const float al = ex2(m - to);
+            m = to;
+            l *= al;
+            if (kt > s.k0) {  // O must hold every earlier tile of the unit
+              if (!__all_sync(0xffffffffu, mbar_wait(&pvdone[q * 2 + ((ns - 1) & 1)], ((ns - 1) >> 1) & 1, abort_flag))) {
+                ok = false;
+                break;
               }
+              fence_after();
 #pragma unroll 1
-              for (int i = 0; i < (kt > s.k0 ? D : 0); i += 8) {
+              for (int i = 0; i < D; i += 8) {
                 uint32_t o[8];
                 ld8(tO + i, o);
 #pragma unroll
@@ -662,19 +669,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
               }
               st_wait();
             }
-            const uint64_t cs2 = pair(cs, cs), nm2 = pair(-m, -m);
+          }
+          const uint64_t cs2 = pair(cs, cs), nm2 = pair(-m, -m);
 #pragma unroll
-            for (int h = 0; h < 64; h += 32) {
-              uint32_t pk[16];
+          for (int h = 0; h < 64; h += 32) {
+            uint32_t pk[16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 v = unpair(fma2(pair(f[h + 2 * i], f[h + 2 * i + 1]), cs2, nm2));
-                const float p0 = ex2(v.x), p1 = ex2(v.y);
-                sum[i & 1] = add2(sum[i & 1], pair(p0, p1));
-                pk[i] = pack_f16(p0, p1);
-              }
-              st16(tS + (c + h) / 2, pk);
+            for (int i = 0; i < 16; ++i) {
+              const float2 v = unpair(fma2(pair(f[h + 2 * i], f[h + 2 * i + 1]), cs2, nm2));
+              const float p0 = ex2(v.x), p1 = ex2(v.y);
+              sum[i & 1] = add2(sum[i & 1], pair(p0, p1));
+              pk[i] = pack_f16(p0, p1);
             }
+            st16(tS + h / 2, pk);
           }
           {
             const float2 a = unpair(sum[0]), b = unpair(sum[1]);
@@ -683,10 +690,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
           st_wait();
           fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&pfull[q]);
+          if (lane == 0) mbar_arrive(&pfull[buf]);
         }
-        if (ok && !__all_sync(0xffffffffu, mbar_wait(&odone[q], no & 1, abort_flag))) ok = false;
-        ++no;
+        if (ok && !__all_sync(0xffffffffu, mbar_wait(&pvdone[q * 2 + ((ns - 1) & 1)], ((ns - 1) >> 1) & 1, abort_flag)))
+          ok = false;
         if (!ok) *abort_flag = 1;
         fence_after();
       }
@@ -694,7 +701,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
       const bool none = s.k0 == s.k1 || !ok;
       const int cta = blockIdx.x;
       auto part = [&](int c, bool head_slot) {
-        return p.part_o + (static_cast<int64_t>(2 * c + (head_slot ? 1 : 0)) * 2 + q) * (D + 2) * 128 + r;
+        return p.part_o + (static_cast<int64_t>(2 * c + (head_slot ? 1 : 0)) * NQ + q) * (D + 2) * 128 + r;
       };
       if (s.whole) {
         const float inv = l == 0.f ? 0.f : p.v_scale / l;  // no key at all: 0 (a NaN stays one)
@@ -840,6 +847,7 @@ extern "C" int sh_paged_attention_fp4_tc(const AttnFp4Params* params, int head_d
   switch (head_dim) {
     case 64: return launch<64>(p, stream);
     case 128: return launch<128>(p, stream);
+    case 256: return launch<256>(p, stream);
     default: return -4;
   }
 }
