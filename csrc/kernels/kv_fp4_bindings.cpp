@@ -198,11 +198,10 @@ void paged_attention_fp4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cac
   const int64_t rows = std::min<int64_t>(max_q_len, 4096) * (hq / hk);  // of one kv head
   int r;
   if (rows > 32 && !invariant) {
-    const int tickets = sh_paged_attention_fp4_tc_tickets();
-    TORCH_CHECK(tickets > 0, who, ": no CUDA device");
-    const Scratch s = scratch(k_cache, stream, sh_paged_attention_fp4_tc_workspace(dim), tickets);
+    const int64_t floats = sh_paged_attention_fp4_tc_workspace(dim);
+    TORCH_CHECK(floats > 0, who, ": no CUDA device");
+    const Scratch s = scratch(k_cache, stream, floats, 0);
     p.part_o = s.part.data_ptr<float>();
-    p.tickets = reinterpret_cast<unsigned*>(s.tickets.data_ptr<int>());
     r = sh_paged_attention_fp4_tc(&p, dim, stream);
   } else {
     // Rows that a CTA holds: as many as the longest query has, up to what its registers carry.

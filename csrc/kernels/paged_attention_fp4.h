@@ -36,8 +36,8 @@ int sh_paged_attention_fp4_ctas(int head_dim, int row_tile);
 int64_t sh_paged_attention_fp4_workspace(int head_dim, int row_tile);
 // 0 on success; head_dim in {64, 128, 256}, block size 64.
 int sh_paged_attention_fp4(const AttnFp4Params* p, int head_dim, int row_tile, cudaStream_t stream);
-// The tensor-core kernel for many query rows: units of 256 rows (128 at head_dim 256), whole_units not supported.
-int sh_paged_attention_fp4_tc_tickets(void);
+// The tensor-core kernel for many query rows: units of 256 rows (128 at head_dim 256), whole_units not supported, no
+// tickets.
 int64_t sh_paged_attention_fp4_tc_workspace(int head_dim);
 int sh_paged_attention_fp4_tc(const AttnFp4Params* p, int head_dim, cudaStream_t stream);
 #ifdef __cplusplus

@@ -5,7 +5,8 @@
 // once per 256 rows (128 at head_dim 256, where two accumulators do not fit TMEM).  The units are laid end to end,
 // each as long as its share of the causal triangle (w_i = (ctx + c) G + (i + 1) ROWS for row tile i, c for a unit's
 // start and end: integers with a closed-form sum, so any place is found by bisection), and cut into one run per SM.  A
-// unit cut by a run's end leaves fp32 partials, merged in order by the last of its CTAs.
+// unit cut by a run's end leaves fp32 partials, which a second kernel merges in order.  (The last CTA of a unit doing
+// it alone, as the short-query kernel does, pulls 133 KB per partial through one SM: 64 tokens over 20000 took 101 us.)
 //
 // Per CTA (512 threads):
 //   warps 0-3, 4-7   one warpgroup per query tile, a row a thread (= its TMEM lane): load the row, scale it by a power
@@ -43,7 +44,8 @@ constexpr int PRODUCERS = 3;  // warps each for K and V
 constexpr int MMA_WARP = 8 + 2 * PRODUCERS;
 constexpr int THREADS = (MMA_WARP + 2) * 32;
 constexpr float kSlack = 8.f;
-constexpr int kUnit = 256;  // a unit's start and end in keys
+constexpr int kMergeDims = 16;
+constexpr int kUnit = 512;  // a unit's start and end in keys (measured: 256 and 1024 leave the SMs less even)
 
 template <int D>
 struct Smem {
@@ -191,6 +193,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ float2 ex2_pair(uint64_t v) {
+  const float2 x = unpair(v);
+  return make_float2(ex2(x.x), ex2(x.y));
+}
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
@@ -234,31 +240,41 @@ struct Segment {
   int b, h, row0, rows, k0, k1;  // key tiles [k0, k1) of the unit
   bool whole, head;              // all of the unit; its beginning
 };
+// Walks a CTA's run [pos, end) of the units laid end to end.  Request b begins at `base`; after the first unit, which
+// is searched for, each one follows from the last without a division.
 struct Cursor {
   int64_t pos, end, base;
-  int b;
+  int b, tile, h;
   Request r;
 };
 template <int ROWS>
 __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, Segment& s) {
   if (c.pos >= c.end) return false;
   const int g = p.hq / p.hk;
-  while (c.pos >= c.base + cost<ROWS>(c.r, g, c.r.tiles) * p.hk) {
-    c.base += cost<ROWS>(c.r, g, c.r.tiles) * p.hk;
-    c.r = request<ROWS>(p, ++c.b);
+  int64_t r0 = 0;
+  if (c.tile < 0) {
+    const int64_t off = c.pos - c.base;
+    int lo = 0, hi = c.r.tiles - 1;  // the tile that holds `off`: its predecessors cost at most that
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cost<ROWS>(c.r, g, mid) * p.hk <= off) lo = mid;
+      else hi = mid - 1;
+    }
+    const int64_t in = off - cost<ROWS>(c.r, g, lo) * p.hk, w = tile_cost<ROWS>(c.r, g, lo);
+    c.tile = lo;
+    c.h = static_cast<int>(in / w);
+    r0 = in % w;
+  } else if (++c.h == p.hk) {
+    c.h = 0;
+    ++c.tile;
+    while (c.tile >= c.r.tiles) {
+      c.r = request<ROWS>(p, ++c.b);
+      c.tile = 0;
+    }
   }
-  const int64_t off = c.pos - c.base;
-  int lo = 0, hi = c.r.tiles - 1;  // the tile that holds `off`: its predecessors cost at most that
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cost<ROWS>(c.r, g, mid) * p.hk <= off) lo = mid;
-    else hi = mid - 1;
-  }
-  const int64_t w = tile_cost<ROWS>(c.r, g, lo);
-  const int64_t in = off - cost<ROWS>(c.r, g, lo) * p.hk;
   s.b = c.b;
-  s.h = static_cast<int>(in / w);
-  s.row0 = lo * ROWS;
+  s.h = c.h;
+  s.row0 = c.tile * ROWS;
   const int64_t left = static_cast<int64_t>(c.r.q_len) * g - s.row0;
   s.rows = left < ROWS ? static_cast<int>(left) : ROWS;
   s.qs = c.r.qs;
@@ -267,16 +283,85 @@ __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, 
   if (kv > c.r.seq) kv = c.r.seq;
   if (kv < 0) kv = 0;
   s.kv_end = kv;
-  const int64_t tiles = (kv + KT - 1) / KT;
-  s.u0 = c.pos - in % w;
+  const int64_t tiles = (kv + KT - 1) / KT, w = tile_cost<ROWS>(c.r, g, c.tile);
+  s.u0 = c.pos - r0;
   s.u1 = s.u0 + w;
-  const int64_t r0 = c.pos - s.u0, r1 = (c.end < s.u1 ? c.end : s.u1) - s.u0;
-  s.k0 = static_cast<int>(r0 * tiles / w);
-  s.k1 = static_cast<int>(r1 * tiles / w);
   s.head = r0 == 0;
-  s.whole = s.head && r1 == w;
-  c.pos = s.u0 + r1;
+  s.whole = s.head && c.end >= s.u1;
+  s.k0 = s.head ? 0 : static_cast<int>(r0 * tiles / w);
+  s.k1 = c.end >= s.u1 ? static_cast<int>(tiles) : static_cast<int>((c.end - s.u0) * tiles / w);
+  c.pos = c.end < s.u1 ? c.end : s.u1;
   return true;
+}
+
+// Run `run` of `runs`: its place among all units and the request it begins in.  Every thread of the block calls it;
+// returns the length of a run.
+template <int ROWS, int N>
+__device__ __forceinline__ int64_t find_run(const AttnFp4Params& p, int run, int runs, Cursor& cur) {
+  __shared__ int64_t scan[N / 32];
+  __shared__ int64_t start_base;
+  __shared__ int start_b;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.hq / p.hk;
+  auto weight = [&](int64_t b) {
+    if (b >= p.B) return int64_t(0);
+    const Request r = request<ROWS>(p, static_cast<int>(b));
+    return cost<ROWS>(r, group, r.tiles) * p.hk;
+  };
+  int64_t total = 0;
+  for (int64_t b = threadIdx.x; b < p.B; b += N) total += weight(b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) scan[warp] = total;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < N / 32; ++w) total += scan[w];
+  __syncthreads();
+  const int64_t per = (total + runs - 1) / runs;
+  cur.pos = per * run;
+  cur.end = cur.pos + per < total ? cur.pos + per : total;
+  cur.tile = -1;
+  if (cur.pos < cur.end) {
+    for (int64_t done = 0, b0 = 0; b0 < p.B; b0 += N) {
+      const int64_t w = weight(b0 + threadIdx.x);
+      int64_t incl = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      int64_t before = done;
+      for (int i = 0; i < warp; ++i) before += scan[i];
+      const int64_t hi = before + incl, lo = hi - w;
+      if (lo <= cur.pos && cur.pos < hi) {
+        start_b = static_cast<int>(b0) + threadIdx.x;
+        start_base = lo;
+      }
+      for (int i = 0; i < N / 32; ++i) done += scan[i];
+      __syncthreads();
+      if (done > cur.pos) break;
+    }
+    cur.b = start_b;
+    cur.base = start_base;
+    cur.r = request<ROWS>(p, cur.b);
+  }
+  return per;
+}
+
+// A unit's partial of run c: O, then the reference and the sum, [D + 2][128] with the row last.  A run leaves two at
+// most, the one that begins in it (and ends later) and the one that began earlier.
+struct Split {
+  int64_t qs;
+  int last, rows, row0, h;  // the run that ends the unit (the own one or less: nothing to merge) and the unit
+};
+template <int D>
+__device__ __forceinline__ Split* splits(const AttnFp4Params& p, int runs) {
+  return reinterpret_cast<Split*>(p.part_o + static_cast<int64_t>(runs) * 2 * Smem<D>::NQ * (D + 2) * 128);
+}
+template <int D>
+__device__ __forceinline__ float* partial(const AttnFp4Params& p, int c, bool begins, int q, int row) {
+  return p.part_o + (static_cast<int64_t>(2 * c + (begins ? 1 : 0)) * Smem<D>::NQ + q) * (D + 2) * 128 + row;
 }
 
 // Eight values, one 16-byte chunk: 8 codes times their block's scale.
@@ -305,11 +390,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
   uint64_t* drain = pvdone + 4;                                  // [q]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* last_flag = abort_flag + 1;  // [2]
-  __shared__ int64_t scan[16];
-  __shared__ int64_t start_base;
-  __shared__ int start_b;
-
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int group = p.hq / p.hk;
   if (threadIdx.x == 0) {
@@ -339,54 +419,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
   shk::pdl_trigger();
   shk::pdl_wait();  // lengths, tables, queries and the new tokens' rows come from earlier kernels
 
-  // ---------------------------------------------------------------- this CTA's run
-  int64_t total = 0;
-  for (int b = threadIdx.x; b < p.B; b += THREADS) {
-    const Request r = request<ROWS>(p, b);
-    total += cost<ROWS>(r, group, r.tiles) * p.hk;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) scan[warp] = total;
-  __syncthreads();
-  total = 0;
-  for (int w = 0; w < THREADS / 32; ++w) total += scan[w];
-  __syncthreads();
-  const int64_t per = (total + gridDim.x - 1) / gridDim.x;
   Cursor cur;
-  cur.pos = per * blockIdx.x;
-  cur.end = cur.pos + per < total ? cur.pos + per : total;
-  if (cur.pos < cur.end) {
-    for (int64_t done = 0, b0 = 0; b0 < p.B; b0 += THREADS) {
-      const int b = static_cast<int>(b0) + threadIdx.x;
-      int64_t w = 0;
-      if (b < p.B) {
-        const Request r = request<ROWS>(p, b);
-        w = cost<ROWS>(r, group, r.tiles) * p.hk;
-      }
-      int64_t incl = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      if (lane == 31) scan[warp] = incl;
-      __syncthreads();
-      int64_t before = done;
-      for (int i = 0; i < warp; ++i) before += scan[i];
-      const int64_t hi = before + incl, lo = hi - w;
-      if (lo <= cur.pos && cur.pos < hi) {
-        start_b = b;
-        start_base = lo;
-      }
-      for (int i = 0; i < THREADS / 32; ++i) done += scan[i];
-      __syncthreads();
-      if (done > cur.pos) break;
-    }
-    cur.b = start_b;
-    cur.base = start_base;
-    cur.r = request<ROWS>(p, cur.b);
-  }
+  const int64_t per = find_run<ROWS, THREADS>(p, blockIdx.x, gridDim.x, cur);
+  if (threadIdx.x == 0) splits<D>(p, gridDim.x)[blockIdx.x].last = -1;
   fence_before();
   __syncthreads();
   fence_after();
@@ -573,46 +608,77 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
     // through the last, so a parity is never two phases old.
     int ns = 0;
     bool ok = true;
-    while (next_segment<ROWS>(p, cur, s)) {
-      if (q * 128 >= s.rows) continue;
-      const int n = q * 128 + r;
-      const bool valid = n < s.rows;
-      const int rr = s.row0 + n;
-      const int64_t tok = s.qs + rr / group;
-      const int head = s.h * group + rr % group;
-      const int64_t pos = s.ctx0 + rr / group;
-      float m = -FLT_MAX, l = 0.f, cs = 0.f;
-      if (s.k0 < s.k1 && ok) {
-        // the query row, its largest element scaled into [2^13, 2^14)
-        uint32_t top = 0;
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + tok * p.q_stride + static_cast<int64_t>(head) * D);
-        uint4 raw[D / 8];
+    // This thread's row of a unit: where it comes from and goes to, its scales, the last key it sees.
+    struct Row {
+      const uint4* src;
+      __nv_bfloat16* dst;
+      int64_t pos;
+      float f, cs;
+      bool valid;
+    };
+    auto advance = [&](Segment& sg) {  // the next unit in which this query tile has rows
+      bool more;
+      do {
+        more = next_segment<ROWS>(p, cur, sg);
+      } while (more && q * 128 >= sg.rows);
+      return more;
+    };
+    auto scan_row = [&](const Segment& sg) {
+      Row w;
+      const int n = q * 128 + r, rr = sg.row0 + n;
+      const int64_t tok = sg.qs + rr / group, col = static_cast<int64_t>(sg.h * group + rr % group) * D;
+      w.valid = n < sg.rows;
+      w.src = reinterpret_cast<const uint4*>(p.q + tok * p.q_stride + col);
+      w.dst = p.out + tok * p.out_stride + col;
+      w.pos = sg.ctx0 + rr / group;
+      uint32_t top = 0;
+      if (w.valid) {
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
-          raw[i] = valid ? src[i] : make_uint4(0, 0, 0, 0);
-          const uint32_t w4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          const uint4 v = w.src[i];
+          const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) top = max(top, max(w4[k] & 0x7fffu, (w4[k] >> 16) & 0x7fffu));
         }
-        const int e = min(267 - static_cast<int>(top >> 7), 253);
-        // the scale's sign goes with the row (0: a zero row), so that cs > 0 and the largest S is the largest score
-        const float f = p.scale_log2 == 0.f ? 0.f : copysignf(__uint_as_float(static_cast<uint32_t>(e) << 23), p.scale_log2);
-        cs = fmaxf(__uint_as_float(static_cast<uint32_t>(254 - e) << 23) * fabsf(p.scale_log2), FLT_MIN);
-        uint8_t* qrow = smem + M::Q + q * M::QTILE + r * 128;
+      }
+      // its largest element goes into [2^13, 2^14); the softmax scale's sign goes with the row (0: a zero row), so that
+      // cs > 0 and the largest S is the largest score
+      const int e = min(267 - static_cast<int>(top >> 7), 253);
+      w.f = p.scale_log2 == 0.f ? 0.f : copysignf(__uint_as_float(static_cast<uint32_t>(e) << 23), p.scale_log2);
+      w.cs = fmaxf(__uint_as_float(static_cast<uint32_t>(254 - e) << 23) * fabsf(p.scale_log2), FLT_MIN);
+      return w;
+    };
+    auto store_row = [&](const Row& w) {
+      uint8_t* qrow = smem + M::Q + q * M::QTILE + r * 128;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint32_t w4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-          uint32_t o[4];
+      for (int i = 0; i < D / 8; ++i) {
+        const uint4 v = w.valid ? w.src[i] : make_uint4(0, 0, 0, 0);  // the scan has left it in L1
+        const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
+        uint32_t o[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            o[k] = pack_f16(__uint_as_float(w4[k] << 16) * f, __uint_as_float(w4[k] & 0xffff0000u) * f);
-          *reinterpret_cast<uint4*>(qrow + (i >> 3) * M::QSLAB + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&qfull[q]);
-
-        const int64_t safe = s.ctx0 + (s.row0 + q * 128) / group;  // the tile's first position
+        for (int k = 0; k < 4; ++k)
+          o[k] = pack_f16(__uint_as_float(w4[k] << 16) * w.f, __uint_as_float(w4[k] & 0xffff0000u) * w.f);
+        *reinterpret_cast<uint4*>(qrow + (i >> 3) * M::QSLAB + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&qfull[q]);
+    };
+    Segment sn;
+    bool have = advance(sn), stored = false;
+    Row next = {};
+    if (have) next = scan_row(sn);
+    while (have) {
+      s = sn;
+      const Row w = next;
+      const float cs = w.cs;
+      float m = -FLT_MAX, l = 0.f;
+      const bool keys = s.k0 < s.k1;
+      if (keys && ok) {
+        if (!stored) store_row(w);
+        // key tiles from here on hold keys that some row of this query tile does not see
+        const int64_t seen = s.ctx0 + (s.row0 + q * 128) / group + 1;
+        const int free_tiles = seen > 0 ? static_cast<int>(seen / KT) : 0;
         for (int kt = s.k0; kt < s.k1; ++kt, ++ns) {
           const int buf = q * 2 + (ns & 1);
           const uint32_t tS = tmem + tl + T_S + buf * KT;
@@ -621,17 +687,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
             break;
           }
           fence_after();
-          const int64_t key0 = static_cast<int64_t>(kt) * KT;
-          const bool edge = key0 + KT - 1 > safe;
-          // keys [0, lim) of the tile are this row's
-          const int lim = edge ? static_cast<int>(min(max(pos + 1 - key0, int64_t(0)), int64_t(KT))) : KT;
           uint64_t sum[2] = {0, 0};
           uint32_t x[64];
           ld32(tS, x);
           ld32(tS + 32, x + 32);
           ld_wait(x);
           ld_wait(x + 32);
-          if (edge) {
+          if (kt >= free_tiles) {
+            // keys [0, lim) of the tile are this row's
+            const int lim = static_cast<int>(min(max(w.pos + 1 - static_cast<int64_t>(kt) * KT, int64_t(0)), int64_t(KT)));
 #pragma unroll
             for (int i = 0; i < 64; ++i)
               if (i >= lim) x[i] = __float_as_uint(-INFINITY);
@@ -676,10 +740,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
             uint32_t pk[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float2 v = unpair(fma2(pair(f[h + 2 * i], f[h + 2 * i + 1]), cs2, nm2));
-              const float p0 = ex2(v.x), p1 = ex2(v.y);
-              sum[i & 1] = add2(sum[i & 1], pair(p0, p1));
-              pk[i] = pack_f16(p0, p1);
+              const uint64_t v = fma2(pair(f[h + 2 * i], f[h + 2 * i + 1]), cs2, nm2);
+              const float2 e = ex2_pair(v);
+              sum[i & 1] = add2(sum[i & 1], pair(e.x, e.y));
+              pk[i] = pack_f16(e.x, e.y);
             }
             st16(tS + h / 2, pk);
           }
@@ -692,20 +756,24 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
           __syncwarp();
           if (lane == 0) mbar_arrive(&pfull[buf]);
         }
+      }
+      // the next unit's row is read while this unit's last product runs, and stored for its MMAs before this one's
+      // results are written
+      have = advance(sn);
+      if (have) next = scan_row(sn);
+      if (keys) {
         if (ok && !__all_sync(0xffffffffu, mbar_wait(&pvdone[q * 2 + ((ns - 1) & 1)], ((ns - 1) >> 1) & 1, abort_flag)))
           ok = false;
         if (!ok) *abort_flag = 1;
         fence_after();
       }
+      stored = have && ok && sn.k0 < sn.k1;
+      if (stored) store_row(next);
       if (!ok) l = __uint_as_float(0x7fc00000u);  // a wait ran out: NaN, not numbers
-      const bool none = s.k0 == s.k1 || !ok;
-      const int cta = blockIdx.x;
-      auto part = [&](int c, bool head_slot) {
-        return p.part_o + (static_cast<int64_t>(2 * c + (head_slot ? 1 : 0)) * NQ + q) * (D + 2) * 128 + r;
-      };
+      const bool none = !keys || !ok;
       if (s.whole) {
         const float inv = l == 0.f ? 0.f : p.v_scale / l;  // no key at all: 0 (a NaN stays one)
-        __nv_bfloat16* dst = p.out + tok * p.out_stride + static_cast<int64_t>(head) * D;
+        __nv_bfloat16* dst = w.dst;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
@@ -716,7 +784,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
             ld32(tO + c, o);
             ld_wait(o);
           }
-          if (valid) {
+          if (w.valid) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               uint32_t v[4];
@@ -729,7 +797,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
         }
         continue;
       }
-      float* mine = part(cta, s.head);
+      if (q == 0 && r == 0 && s.head)
+        splits<D>(p, gridDim.x)[blockIdx.x] = {s.qs, static_cast<int>((s.u1 - 1) / per), s.rows, s.row0, s.h};
+      float* mine = partial<D>(p, blockIdx.x, s.head, q, r);
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -745,45 +815,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
       }
       mine[D * 128] = m;
       mine[(D + 1) * 128] = l;
-      __threadfence();
-      named_barrier(1 + q, 128);
-      const int first = static_cast<int>(s.u0 / per), last = static_cast<int>((s.u1 - 1) / per);
-      if (r == 0) {
-        unsigned* ticket = p.tickets + 2 * first + q;
-        const bool is_last = atomicAdd(ticket, 1u) == static_cast<unsigned>(last - first);
-        last_flag[q] = is_last;
-        if (is_last) *ticket = 0;
-        __threadfence();
-      }
-      named_barrier(1 + q, 128);
-      if (last_flag[q]) {
-        float top = -FLT_MAX, den = 0.f;
-        for (int c = first; c <= last; ++c) top = fmaxf(top, __ldcg(part(c, c == first) + D * 128));
-        for (int c = first; c <= last; ++c)
-          den += ex2(__ldcg(part(c, c == first) + D * 128) - top) * __ldcg(part(c, c == first) + (D + 1) * 128);
-        const float inv = den == 0.f ? 0.f : p.v_scale / den;
-        __nv_bfloat16* dst = p.out + tok * p.out_stride + static_cast<int64_t>(head) * D;
-#pragma unroll 1
-        for (int d = 0; d < D; d += 16) {
-          float acc[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) acc[k] = 0.f;
-          for (int c = first; c <= last; ++c) {
-            const float* src = part(c, c == first);
-            const float wt = ex2(__ldcg(src + D * 128) - top);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) acc[k] += wt * __ldcg(src + (d + k) * 128);
-          }
-          if (valid) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              *reinterpret_cast<uint4*>(dst + d + 8 * k) =
-                  make_uint4(pack_bf16(acc[8 * k] * inv, acc[8 * k + 1] * inv), pack_bf16(acc[8 * k + 2] * inv, acc[8 * k + 3] * inv),
-                             pack_bf16(acc[8 * k + 4] * inv, acc[8 * k + 5] * inv), pack_bf16(acc[8 * k + 6] * inv, acc[8 * k + 7] * inv));
-          }
-        }
-      }
-      named_barrier(1 + q, 128);  // last_flag is rewritten by the next unit
     }
   }
   fence_before();
@@ -792,6 +823,53 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(T_COLS));
   }
+}
+
+// The unit that run blockIdx.x begins and a later one ends, if there is one: its partials, in order.  blockIdx.y: query
+// tile and kMergeDims of the dimensions; a thread holds a row.
+template <int D>
+__global__ void __launch_bounds__(128) merge_kernel(AttnFp4Params p, int runs) {
+  constexpr int DC = kMergeDims;
+  shk::pdl_trigger();
+  shk::pdl_wait();
+  const int q = blockIdx.y / (D / DC), d0 = blockIdx.y % (D / DC) * DC, r = threadIdx.x;
+  const Split s = splits<D>(p, runs)[blockIdx.x];
+  const int first = blockIdx.x, last = s.last;
+  if (last <= first || q * 128 + r >= s.rows) return;
+  float top = -FLT_MAX, den = 0.f, acc[DC];
+#pragma unroll
+  for (int k = 0; k < DC; ++k) acc[k] = 0.f;
+#pragma unroll 8
+  for (int c = first; c <= last; ++c) top = fmaxf(top, __ldcg(partial<D>(p, c, c == first, q, r) + D * 128));
+  constexpr int BATCH = 4;  // partials whose loads are in flight together
+  for (int c0 = first; c0 <= last; c0 += BATCH) {
+    float v[BATCH][DC], m[BATCH], l[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int c = c0 + i <= last ? c0 + i : last;
+      const float* src = partial<D>(p, c, c == first, q, r);
+      m[i] = __ldcg(src + D * 128);
+      l[i] = __ldcg(src + (D + 1) * 128);
+#pragma unroll
+      for (int k = 0; k < DC; ++k) v[i][k] = __ldcg(src + (d0 + k) * 128);
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      if (c0 + i > last) break;
+      const float wt = ex2(m[i] - top);
+      den += wt * l[i];
+#pragma unroll
+      for (int k = 0; k < DC; ++k) acc[k] += wt * v[i][k];
+    }
+  }
+  const float inv = den == 0.f ? 0.f : p.v_scale / den;  // no key at all: 0 (a NaN stays one)
+  const int group = p.hq / p.hk, rr = s.row0 + q * 128 + r;
+  __nv_bfloat16* dst = p.out + (s.qs + rr / group) * p.out_stride + static_cast<int64_t>(s.h * group + rr % group) * D + d0;
+#pragma unroll
+  for (int k = 0; k < DC; k += 8)
+    *reinterpret_cast<uint4*>(dst + k) =
+        make_uint4(pack_bf16(acc[k] * inv, acc[k + 1] * inv), pack_bf16(acc[k + 2] * inv, acc[k + 3] * inv),
+                   pack_bf16(acc[k + 4] * inv, acc[k + 5] * inv), pack_bf16(acc[k + 6] * inv, acc[k + 7] * inv));
 }
 
 }  // namespace attn4tc
@@ -824,22 +902,21 @@ int launch(const AttnFp4Params& p, cudaStream_t st) {
   }
   const int ctas = num_sms();
   if (ctas <= 0) return -5;
-  const cudaError_t e = shk::launch(k, dim3(ctas), dim3(THREADS), Smem<D>::TOTAL, st, p);
+  cudaError_t e = shk::launch(k, dim3(ctas), dim3(THREADS), Smem<D>::TOTAL, st, p);
+  if (e == cudaSuccess) e = shk::launch(merge_kernel<D>, dim3(ctas, Smem<D>::NQ * D / kMergeDims), dim3(128), 0, st, p, ctas);
   return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
 }
 }  // namespace
 
-extern "C" int sh_paged_attention_fp4_tc_tickets(void) { return 2 * num_sms(); }
-
 extern "C" int64_t sh_paged_attention_fp4_tc_workspace(int head_dim) {
-  return static_cast<int64_t>(num_sms()) * 4 * (head_dim + 2) * 128;
+  return static_cast<int64_t>(num_sms()) * (4 * (head_dim + 2) * 128 + sizeof(Split) / 4);
 }
 
 extern "C" int sh_paged_attention_fp4_tc(const AttnFp4Params* params, int head_dim, cudaStream_t stream) {
   const AttnFp4Params& p = *params;
   if (p.num_tokens <= 0 || p.B <= 0) return 0;
   if (p.hk <= 0 || p.hq % p.hk != 0 || p.num_blocks <= 0 || p.bt_cols <= 0 || p.whole_units) return -1;
-  if (p.part_o == nullptr || p.tickets == nullptr) return -2;
+  if (p.part_o == nullptr) return -2;
   if ((reinterpret_cast<uintptr_t>(p.k_cache) & 15) || (reinterpret_cast<uintptr_t>(p.v_cache) & 15) ||
       (reinterpret_cast<uintptr_t>(p.q) & 15) || (p.q_stride & 7) || (reinterpret_cast<uintptr_t>(p.out) & 15) ||
       (p.out_stride & 7))
