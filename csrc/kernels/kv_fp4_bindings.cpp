@@ -204,8 +204,10 @@ void paged_attention_fp4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cac
     p.part_o = s.part.data_ptr<float>();
     r = sh_paged_attention_fp4_tc(&p, dim, stream);
   } else {
-    // Rows that a CTA holds: as many as the longest query has, up to what its registers carry.
-    const int tile = static_cast<int>(std::min<int64_t>((rows + 7) / 8 * 8, d == 256 ? 16 : 32));
+    // Rows that a CTA holds: as many as the longest query has, up to what its registers carry.  Tiles of different
+    // sizes deal the keys to their warps differently, so batch-invariant calls always take the largest.
+    const int most = d == 256 ? 16 : 32;
+    const int tile = invariant ? most : static_cast<int>(std::min<int64_t>((rows + 7) / 8 * 8, most));
     const int ctas = sh_paged_attention_fp4_ctas(dim, tile);
     TORCH_CHECK(ctas > 0, who, ": no CUDA device");
     const Scratch s = scratch(k_cache, stream, sh_paged_attention_fp4_workspace(dim, tile), ctas);

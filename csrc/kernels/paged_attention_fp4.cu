@@ -10,10 +10,10 @@
 // fp32 partial (O, max, sum); the last of its CTAs to finish (a ticket, which it resets) merges them in page order,
 // so the result does not depend on the order of arrival.
 //
-// A CTA's 8 warps take the run's 16-token chunks in turn, each through a ring of its own in shared memory, filled
-// with cp.async three chunks ahead: no barrier between the warps while they stream.  Per chunk and warp, with
-// m16n8k16 (f16 in, fp32 out) and the KEYS on the M side, so 8 query rows fill the N side that decode has:
-//   S^T (16 tokens x rows) = K Q^T,   O^T (D x rows) += V^T P^T.
+// A CTA's warps take the run's 32-token chunks in turn, each through a ring of its own in shared memory, filled with
+// cp.async: no barrier between the warps while they stream.  Per chunk and warp, with m16n8k16 (f16 in, fp32 out) and
+// the KEYS on the M side, so 8 query rows fill the N side that decode has:
+//   S^T (tokens x rows) = K Q^T,   O^T (D x rows) += V^T P^T.
 // Both products are free to permute the dimension they sum over, or the rows of the result: thread (g, t) of the
 // quad layout takes D/4 consecutive dimensions of a key as its share of K's columns, and D/8 consecutive dimensions
 // as its share of V^T's rows, so its codes are one 8- to 32-byte run of a row and one or two scales cover them.
@@ -40,39 +40,59 @@
 namespace shk {
 namespace attn4 {
 
-constexpr int WARPS = 8;
-constexpr int THREADS = WARPS * 32;
-constexpr int CHUNK = 16;  // tokens of one warp step
-constexpr int PAGE = 64;   // tokens of a page
+constexpr int PAGE = 64;  // tokens of a page
 constexpr float kSlack = 8.f;
-constexpr int kMinPages = 2;  // shortest run: a chunk for every warp
+constexpr int kMinPages = 2;  // shortest run
 
 template <int D>
 struct Geo {
   static constexpr int ROW = D / 2;              // code bytes of a token
   static constexpr int SROW = D / 16;            // scale bytes of a token
   static constexpr int PAGE_BYTES = PAGE * (ROW + SROW);
-  static constexpr int CODES = CHUNK * ROW;
-  static constexpr int SCALES = CHUNK * SROW;
-  static constexpr int STAGE = 2 * (CODES + SCALES);
   static constexpr int PIECES = ROW / 16;        // 16-byte pieces of a token's codes
 };
+// Warps of a CTA, CTAs of an SM, 16-token groups of a warp step (a chunk) and ring stages.  O^T takes D / 4 registers a
+// thread for every 8 rows: one row tile of 8 leaves room for two CTAs of 8 warps (128 registers a thread), more for one
+// CTA of 12 (168) or 8 warps (255).
 template <int D, int NT>
 struct Cfg {
-  static constexpr int CTAS = (D <= 128 && NT == 1) ? 2 : 1;  // per SM
-  static constexpr int STAGES = CTAS == 2 ? 4 : (D == 256 ? 3 : 6);
+  static constexpr int REGS_O = D / 4 * NT;
+  static constexpr int SUB = NT == 1 ? 2 : 1;
+  static constexpr int CTAS = REGS_O <= 32 ? 2 : 1;
+  static constexpr int WARPS = REGS_O <= 32 ? 8 : (REGS_O <= 96 ? 12 : 8);
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int CHUNK = 16 * SUB;
+  static constexpr int CODES = CHUNK * Geo<D>::ROW;
+  static constexpr int SCALES = CHUNK * Geo<D>::SROW;
+  static constexpr int STAGE = 2 * (CODES + SCALES);
   static constexpr int MSTRIDE = D + 4;  // floats of a merge row
-  static constexpr int RING = WARPS * STAGES * Geo<D>::STAGE;
   static constexpr int MERGE = WARPS * 8 * MSTRIDE * 4;
-  static constexpr int STATS = 2 * WARPS * 8 * NT * 4;
-  static constexpr int SMEM = RING + MERGE + STATS;
+  static constexpr int QUERY = NT * D * 16;  // the row tile's fragments
+  static constexpr int STATS = 2 * WARPS * 8 * NT * 4 + 2 * 8 * NT * 4;
+  static constexpr int ROOM = 225 * 1024 / CTAS - QUERY - STATS;
+  // with two stages that leave no room for the merge area, it takes the ring's place after each unit
+  static constexpr bool SHARED = 2 * WARPS * STAGE + MERGE > ROOM;
+  static constexpr int FIT = (SHARED ? ROOM : ROOM - MERGE) / (WARPS * STAGE);
+  static constexpr int STAGES = FIT < 6 ? FIT : 6;
+  static constexpr int RING = WARPS * STAGES * STAGE;
+  static constexpr int SMEM = (SHARED ? (RING > MERGE ? RING : MERGE) : RING + MERGE) + QUERY + STATS;
+  static_assert(STAGES >= 2, "a chunk in flight while another is used");
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
+template <int DST, int SRC>
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
+}
+// Pieces I, I + 1, ... < N of this lane, 512 bytes apart on both sides; the odd ones go to another base.
+template <int I, int N>
+__device__ __forceinline__ void cp_pieces(uint32_t even, uint32_t odd, const void* src) {
+  if constexpr (I < N) {
+    cp16<512 * I, 512 * I>(I & 1 ? odd : even, src);
+    cp_pieces<I + 1, N>(even, odd, src);
+  }
 }
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -138,8 +158,8 @@ __device__ __forceinline__ int value_at(int r, int p) {
 
 // What a request asks for, clipped to the tensors it indexes.
 struct Request {
-  int64_t qs, seq;
-  int q_len, tiles, pages;
+  int64_t qs;
+  int seq, q_len, tiles, pages;
 };
 __device__ __forceinline__ Request request(const AttnFp4Params& p, int b, int rows) {
   Request r;
@@ -147,12 +167,12 @@ __device__ __forceinline__ Request request(const AttnFp4Params& p, int b, int ro
   r.qs = q0 < 0 ? 0 : q0;
   const int64_t n = (q1 < p.num_tokens ? q1 : p.num_tokens) - r.qs;
   r.q_len = n > 0 ? static_cast<int>(n) : 0;
-  r.seq = p.seq_lens[b];
-  if (r.seq < 0) r.seq = 0;
-  const int64_t cap = static_cast<int64_t>(p.bt_cols) * PAGE;
-  if (r.seq > cap) r.seq = cap;
+  int64_t seq = p.seq_lens[b];
+  if (seq < 0) seq = 0;
+  const int64_t cap = static_cast<int64_t>(p.bt_cols) * PAGE;  // below 2^31
+  r.seq = static_cast<int>(seq < cap ? seq : cap);
   r.tiles = static_cast<int>((static_cast<int64_t>(r.q_len) * (p.hq / p.hk) + rows - 1) / rows);
-  r.pages = static_cast<int>((r.seq + PAGE - 1) / PAGE);
+  r.pages = (r.seq + (PAGE - 1)) / PAGE;
   if (r.pages < 1) r.pages = 1;  // a request without keys still has its rows to write
   return r;
 }
@@ -163,71 +183,85 @@ __device__ __forceinline__ int64_t weight(const AttnFp4Params& p, const Request&
 // One unit's part in a CTA's run.
 struct Segment {
   int64_t u0, u1;  // the unit's place among all pages
-  int b, h, row0, pg0, pg1, pages, c0, c1;  // c0, c1: chunks with keys that some row sees
-  int64_t qs, ctx0, kv_end;
-  int rows;
+  int64_t qs;
+  int b, h, row0, rows, ctx0, kv_end;
+  int pg0, c0, c1;  // first page; chunks with keys that some row sees
+  bool whole;       // all of the unit
 };
-// Walks a CTA's run [pos, end) of the pages laid end to end; `base` is the place of request b's first page.
+// Walks a CTA's run [pos, end) of the pages laid end to end.  Request b's first page is at `base`; after the first unit
+// each one follows from the last without a division.
 struct Cursor {
   int64_t pos, end, base;
-  int b;
+  int b, tile, h;
   Request r;
 };
-template <int ROWS>
+template <int ROWS, int CHUNK>
 __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, Segment& s) {
   const int g = p.hq / p.hk;
-  int64_t unit;
-  while (true) {
+  int off = 0;  // pages of the unit that belong to an earlier run
+  if (c.tile < 0) {
     if (c.pos >= c.end) return false;
-    while (c.pos >= c.base + weight(p, c.r)) {
-      c.base += weight(p, c.r);
-      c.r = request(p, ++c.b, ROWS);
+    const int64_t unit = (c.pos - c.base) / c.r.pages;
+    off = static_cast<int>((c.pos - c.base) % c.r.pages);
+    c.tile = static_cast<int>(unit / p.hk);
+    c.h = static_cast<int>(unit % p.hk);
+    if (p.whole_units && off) {  // it belongs to the run that it begins in
+      c.pos += c.r.pages - off;
+      off = 0;
+      ++c.h;
     }
-    unit = (c.pos - c.base) / c.r.pages;
-    const int64_t at = c.base + unit * c.r.pages;
-    if (!p.whole_units || at == c.pos) break;
-    c.pos = at + c.r.pages;  // whole units: one that began in an earlier run belongs to that run's CTA
+  } else {
+    ++c.h;
+  }
+  if (c.pos >= c.end) return false;
+  if (c.h == p.hk) {
+    c.h = 0;
+    ++c.tile;
+  }
+  while (c.tile >= c.r.tiles) {
+    c.r = request(p, ++c.b, ROWS);
+    c.tile = 0;
   }
   s.b = c.b;
-  s.h = static_cast<int>(unit % p.hk);
-  const int tile = static_cast<int>(unit / p.hk);
-  s.row0 = tile * ROWS;
+  s.h = c.h;
+  s.row0 = c.tile * ROWS;
   const int64_t left = static_cast<int64_t>(c.r.q_len) * g - s.row0;
   s.rows = left < ROWS ? static_cast<int>(left) : ROWS;
-  s.u0 = c.base + unit * c.r.pages;
+  s.u0 = c.pos - off;
   s.u1 = s.u0 + c.r.pages;
-  s.pages = c.r.pages;
-  s.pg0 = static_cast<int>(c.pos - s.u0);
-  s.pg1 = p.whole_units || c.end >= s.u1 ? c.r.pages : static_cast<int>(c.end - s.u0);
-  c.pos = s.u0 + s.pg1;
+  s.pg0 = off;
+  const bool to_end = p.whole_units || c.end >= s.u1;
+  const int pg1 = to_end ? c.r.pages : static_cast<int>(c.end - s.u0);
+  s.whole = off == 0 && to_end;
+  c.pos = s.u0 + pg1;
   s.qs = c.r.qs;
   s.ctx0 = c.r.seq - c.r.q_len;
-  int64_t kv = s.ctx0 + (s.row0 + s.rows - 1) / g + 1;  // keys the tile's last row sees
-  if (kv > c.r.seq) kv = c.r.seq;
-  if (kv < 0) kv = 0;
+  int kv = s.ctx0 + (s.row0 + s.rows - 1) / g + 1;  // keys the tile's last row sees
+  kv = kv < 0 ? 0 : (kv < c.r.seq ? kv : c.r.seq);
   s.kv_end = kv;
-  const int64_t last = (kv + CHUNK - 1) / CHUNK;
-  s.c0 = s.pg0 * (PAGE / CHUNK);
-  s.c1 = s.pg1 * (PAGE / CHUNK);
-  if (s.c1 > last) s.c1 = static_cast<int>(last);
+  s.c0 = off * (PAGE / CHUNK);
+  const int last = kv / CHUNK + (kv % CHUNK ? 1 : 0);
+  s.c1 = pg1 * (PAGE / CHUNK) < last ? pg1 * (PAGE / CHUNK) : last;
   return true;
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(AttnFp4Params p) {
+__global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(AttnFp4Params p) {
   using G = Geo<D>;
   using K = Cfg<D, NT>;
-  constexpr int ROWS = 8 * NT;
-  constexpr int STAGES = K::STAGES;
-  constexpr int KSTEPS = D / 16;
-  constexpr int MT = D / 16;
-  constexpr int KW = D / 32;  // words of a key in a thread (D/4 codes)
-  constexpr int VB = D / 16;  // bytes of a value in a thread (D/8 codes)
+  constexpr int ROWS = 8 * NT, WARPS = K::WARPS, THREADS = K::THREADS, STAGES = K::STAGES;
+  constexpr int CHUNK = K::CHUNK, SUB = K::SUB;
+  constexpr int MT = D / 16;  // M tiles of O^T
+  constexpr int KW = D / 32;  // words of a key in a thread (D/4 codes), two k-steps each
+  constexpr int VW = D / 64;  // words of a value in a thread (D/8 codes), four M tiles each
   extern __shared__ __align__(128) uint8_t smem[];
-  float* merge_o = reinterpret_cast<float*>(smem + K::RING);
-  float* merge_m = reinterpret_cast<float*>(smem + K::RING + K::MERGE);  // [WARPS][ROWS]
+  float* merge_o = reinterpret_cast<float*>(smem + (K::SHARED ? 0 : K::RING));
+  uint4* query = reinterpret_cast<uint4*>(smem + K::SMEM - K::STATS - K::QUERY);  // [NT][KW][32 lanes]
+  float* merge_m = reinterpret_cast<float*>(smem + K::SMEM - K::STATS);           // [WARPS][ROWS]
   float* merge_l = merge_m + WARPS * ROWS;
-  __shared__ int64_t scan[WARPS + 1];
+  float* row_scale = merge_l + WARPS * ROWS;           // [ROWS]
+  int* row_pos = reinterpret_cast<int*>(row_scale + ROWS);  // [ROWS] last key a row sees
+  __shared__ int64_t scan[WARPS];
   __shared__ int64_t start_base;
   __shared__ int start_b;
   __shared__ int last_flag;
@@ -279,76 +313,92 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
   }
   cons.b = start_b;
   cons.base = start_base;
+  cons.tile = -1;
   cons.r = request(p, cons.b, ROWS);
 
   // ---------------------------------------------------------------- loads of this warp's chunks
-  const uint32_t ring = smem_addr(smem) + warp * STAGES * G::STAGE;
+  const uint32_t ring = smem_addr(smem) + warp * STAGES * K::STAGE;
+  // where this lane's pieces of a chunk go: piece i * 32 + lane is row i * 512 / ROW + lane / PIECES
+  const uint32_t kdst = ring + key_at<D>(lane / G::PIECES, lane % G::PIECES);
+  const uint32_t vdst = ring + K::CODES + value_at<D>(lane / G::PIECES, lane % G::PIECES);
   Cursor prod = cons;
-  Segment ps;
-  bool pmore = next_segment<ROWS>(p, prod, ps);
-  int pc = pmore ? ps.c0 + warp : 0;
-  int page = 0;  // cache block of chunk pc, fetched one chunk ahead of its use
-  auto settle = [&]() {  // moves pc to this warp's next chunk and looks its block up
-    while (pmore && pc >= ps.c1) {
-      pmore = next_segment<ROWS>(p, prod, ps);
-      pc = ps.c0 + warp;
-    }
-    if (pmore) {
-      page = p.block_tables[static_cast<int64_t>(ps.b) * p.bt_stride + pc / (PAGE / CHUNK)];
-      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) page = 0;
-    }
+  bool pmore = false;
+  int pc = 0, pc1 = 0, page = 0;  // this warp's next chunk, the segment's end, the chunk's cache block
+  const int32_t* table = nullptr;
+  int64_t head = 0;  // the segment's head inside a block
+  auto look_up = [&]() {
+    page = table[pc / (PAGE / CHUNK)];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) page = 0;
+  };
+  auto begin = [&](const Segment& sg) {
+    pc = sg.c0 + warp;
+    pc1 = sg.c1;
+    table = p.block_tables + static_cast<int64_t>(sg.b) * p.bt_stride;
+    head = static_cast<int64_t>(sg.h) * G::PAGE_BYTES;
+    pmore = pc < pc1;
+    if (pmore) look_up();
+  };
+  auto settle = [&]() {  // the next segment with a chunk for this warp
+    Segment sg;
+    do {
+      if (!next_segment<ROWS, CHUNK>(p, prod, sg)) {
+        pmore = false;
+        return;
+      }
+    } while (sg.c0 + warp >= sg.c1);
+    begin(sg);
   };
   auto fetch = [&](int stage) {
     if (pmore) {
-      const int64_t off = (static_cast<int64_t>(page) * p.hk + ps.h) * G::PAGE_BYTES;
-      const int sub = pc % (PAGE / CHUNK);
-      const uint32_t dst = ring + stage * G::STAGE;
-      const uint8_t* kc = p.k_cache + off + sub * G::CODES;
-      const uint8_t* vc = p.v_cache + off + sub * G::CODES;
-#pragma unroll
-      for (int i = 0; i < CHUNK * G::PIECES / 32; ++i) {
-        const int idx = i * 32 + lane, r = idx / G::PIECES, q = idx % G::PIECES;
-        cp16(dst + key_at<D>(r, q), kc + idx * 16);
-        cp16(dst + G::CODES + value_at<D>(r, q), vc + idx * 16);
-      }
+      const int64_t off = static_cast<int64_t>(page) * p.hk * G::PAGE_BYTES + head;
+      const int part = pc % (PAGE / CHUNK);
+      const uint32_t kd = kdst + stage * K::STAGE, vd = vdst + stage * K::STAGE;
+      cp_pieces<0, K::CODES / 512>(kd, kd, p.k_cache + off + part * K::CODES + lane * 16);
+      // head_dim 256: a value row's place in its line turns with every second row, so with every second piece
+      cp_pieces<0, K::CODES / 512>(vd, D == 256 ? vd ^ 64 : vd, p.v_cache + off + part * K::CODES + lane * 16);
+      constexpr int N = K::SCALES / 16;  // pieces of the scales: the keys' for the first half of the warp
       const int half = lane >> 4, i = lane & 15;
-      if (i < G::SCALES / 16)
-        cp16(dst + 2 * G::CODES + half * G::SCALES + i * 16,
-             (half ? p.v_cache : p.k_cache) + off + PAGE * G::ROW + sub * G::SCALES + i * 16);
+      const uint8_t* sc = (half ? p.v_cache : p.k_cache) + off + PAGE * G::ROW + part * K::SCALES + i * 16;
+      const uint32_t sd = ring + stage * K::STAGE + 2 * K::CODES + half * K::SCALES + i * 16;
+      if (i < N) cp16<0, 0>(sd, sc);
+      if constexpr (N > 16) cp16<256, 256>(sd, sc);
       pc += WARPS;
-      settle();
+      if (pc < pc1) look_up();
+      else if constexpr (K::SHARED) pmore = false;
+      else settle();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  settle();
+  if constexpr (!K::SHARED) {
+    settle();
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) fetch(s);
+    for (int st = 0; st < STAGES - 1; ++st) fetch(st);
+  }
+  int it = 0;
+
+  // per-lane places of the fragments in a chunk: keys g (+ 8, ...), values 2 t and 2 t + 1 (+ 8, ...)
+  const int koff0 = key_at<D>(g, D == 64 ? t >> 1 : t * (D / 128)) + (D == 64 ? (t & 1) * 8 : 0);
+  const int koff1 = D == 256 ? key_at<D>(g, t * 2 + 1) : 0;
+  const int vp = D == 256 ? g : (D == 128 ? g >> 1 : g >> 2), vb = D == 256 ? 0 : (D == 128 ? (g & 1) * 8 : (g & 3) * 4);
+  const int voff0 = K::CODES + value_at<D>(2 * t, vp) + vb, voff1 = K::CODES + value_at<D>(2 * t + 1, vp) + vb;
+  const int ksoff = 2 * K::CODES + g * G::SROW + t * (D / 64);
+  const int vsoff = 2 * K::CODES + K::SCALES + 2 * t * G::SROW + (D == 64 ? g >> 1 : (D == 128 ? g : 2 * g));
 
   // ---------------------------------------------------------------- segments
-  int it = 0;
   Segment s;
-  while (next_segment<ROWS>(p, cons, s)) {
-    uint32_t qf[NT][KSTEPS][2];
-    float cs[NT][2], m[NT][2], l[NT][2];
-    int64_t pos[NT][2];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int n = 8 * j + g;
-      float f = 1.f, inv = 1.f;
+  while (next_segment<ROWS, CHUNK>(p, cons, s)) {
+    // The row tile's fragments, a warp per 8 rows: lane (g, t) has dimensions [t D/4, (t + 1) D/4) of row g, word u of
+    // its codes against query[j][u][lane].
+#pragma unroll 1
+    for (int j = warp; j < NT; j += WARPS) {
+      const int n = 8 * j + g, rr = s.row0 + n;
       uint4 raw[D / 32];
-      if (n < s.rows) {
-        const int rr = s.row0 + n;
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + (s.qs + rr / group) * p.q_stride +
-                                                          static_cast<int64_t>(s.h * group + rr % group) * D + t * (D / 4));
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) raw[i] = src[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) raw[i] = make_uint4(0, 0, 0, 0);
-      }
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (s.qs + rr / group) * p.q_stride +
+                                                        static_cast<int64_t>(s.h * group + rr % group) * D + t * (D / 4));
       uint32_t top = 0;  // largest magnitude's bf16 bits: its exponent is all that is needed
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
+        raw[i] = n < s.rows ? src[i] : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
@@ -356,25 +406,36 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = min(267 - static_cast<int>(top >> 7), 253);  // biased exponent of the row's factor
-      f = __uint_as_float(static_cast<uint32_t>(e) << 23);
-      inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * p.scale_log2;
+      const float f = __uint_as_float(static_cast<uint32_t>(e) << 23);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        uint32_t o[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          qf[j][2 * i + k / 2][k & 1] =
-              pack_f16(__uint_as_float(w[k] << 16) * f, __uint_as_float(w[k] & 0xffff0000u) * f);
+        for (int k = 0; k < 4; ++k) o[k] = pack_f16(__uint_as_float(w[k] << 16) * f, __uint_as_float(w[k] & 0xffff0000u) * f);
+        query[(j * KW + i) * 32 + lane] = make_uint4(o[0], o[1], o[2], o[3]);
       }
-#pragma unroll
-      for (int e2 = 0; e2 < 2; ++e2) {
-        cs[j][e2] = __shfl_sync(0xffffffffu, inv, (2 * t + e2) * 4);
-        pos[j][e2] = s.ctx0 + (s.row0 + 8 * j + 2 * t + e2) / group;
-        m[j][e2] = -FLT_MAX;
-        l[j][e2] = 0.f;
+      if (t == 0) {
+        row_scale[n] = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * p.scale_log2;
+        row_pos[n] = s.ctx0 + rr / group;
       }
     }
-    const int64_t safe = s.ctx0 + s.row0 / group;  // the tile's first position: keys up to it need no mask
+    if constexpr (K::SHARED) {
+      begin(s);
+#pragma unroll
+      for (int st = 0; st < STAGES - 1; ++st) fetch((it + st) % STAGES);
+    }
+    __syncthreads();
+    float cs[NT][2], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        cs[j][e] = row_scale[8 * j + 2 * t + e];
+        m[j][e] = -FLT_MAX;
+        l[j][e] = 0.f;
+      }
+    const int safe = row_pos[0];  // the tile's first position: keys up to it need no mask
     float o[NT][MT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -386,34 +447,36 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
       __syncwarp();
       fetch((it + STAGES - 1) % STAGES);
-      const uint8_t* st = smem + warp * STAGES * G::STAGE + (it % STAGES) * G::STAGE;
-      const int64_t key0 = static_cast<int64_t>(c) * CHUNK;
+      const uint8_t* st = smem + warp * STAGES * K::STAGE + (it % STAGES) * K::STAGE;
+      const int key0 = c * CHUNK;
       const bool edge = key0 + CHUNK - 1 > safe;
       // -------- S^T = K Q^T
-      float sc[NT][4];
+      float sc[SUB][NT][4];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sc[u][j][0] = sc[u][j][1] = sc[u][j][2] = sc[u][j][3] = 0.f;
       {
-        uint32_t kw[2][KW];
-        uint32_t ksc[2][D / 64];  // the scale of each 16 dimensions, twice
+        uint32_t kw[2 * SUB][KW];
+        uint32_t ksc[2 * SUB][D / 64];  // the scale of each 16 dimensions, twice
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int r = g + 8 * hf;
+        for (int hf = 0; hf < 2 * SUB; ++hf) {  // rows g + 8 hf
+          const uint8_t* kp = st + koff0 + 8 * hf * G::ROW;
           if constexpr (D == 64) {
-            const uint2 v = *reinterpret_cast<const uint2*>(st + key_at<D>(r, t >> 1) + (t & 1) * 8);
+            const uint2 v = *reinterpret_cast<const uint2*>(kp);
             kw[hf][0] = v.x;
             kw[hf][1] = v.y;
           } else {
 #pragma unroll
             for (int i = 0; i < D / 128; ++i) {
-              const uint4 v = *reinterpret_cast<const uint4*>(st + key_at<D>(r, t * (D / 128) + i));
+              const uint4 v = *reinterpret_cast<const uint4*>(i ? st + koff1 + 8 * hf * G::ROW : kp);
               kw[hf][4 * i] = v.x;
               kw[hf][4 * i + 1] = v.y;
               kw[hf][4 * i + 2] = v.z;
               kw[hf][4 * i + 3] = v.w;
             }
           }
-          const uint8_t* sp = st + 2 * G::CODES + r * G::SROW + t * (D / 64);
+          const uint8_t* sp = st + ksoff + 8 * hf * G::SROW;
           uint32_t w;
           if constexpr (D == 64) w = *sp;
           if constexpr (D == 128) w = *reinterpret_cast<const uint16_t*>(sp);
@@ -427,30 +490,61 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
         }
 #pragma unroll
         for (int w = 0; w < KW; ++w) {  // 8 codes: two k-steps
-          uint32_t lo[4], hi[4];
-          e2m1x8(kw[0][w], lo);
-          e2m1x8(kw[1][w], hi);
+          uint4 qf[NT];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t a[4] = {hmul2(lo[2 * k], ksc[0][w / 2]), hmul2(hi[2 * k], ksc[1][w / 2]),
-                                   hmul2(lo[2 * k + 1], ksc[0][w / 2]), hmul2(hi[2 * k + 1], ksc[1][w / 2])};
+          for (int j = 0; j < NT; ++j) qf[j] = query[(j * KW + w) * 32 + lane];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma(sc[j], a, qf[j][2 * w + k][0], qf[j][2 * w + k][1]);
+          for (int u = 0; u < SUB; ++u) {
+            uint32_t lo[4], hi[4];
+            e2m1x8(kw[2 * u][w], lo);
+            e2m1x8(kw[2 * u + 1][w], hi);
+            const uint32_t s0 = ksc[2 * u][w / 2], s1 = ksc[2 * u + 1][w / 2];
+            const uint32_t a0[4] = {hmul2(lo[0], s0), hmul2(hi[0], s1), hmul2(lo[1], s0), hmul2(hi[1], s1)};
+            const uint32_t a1[4] = {hmul2(lo[2], s0), hmul2(hi[2], s1), hmul2(lo[3], s0), hmul2(hi[3], s1)};
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma(sc[u][j], a0, qf[j].x, qf[j].y);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma(sc[u][j], a1, qf[j].z, qf[j].w);
           }
         }
       }
       // -------- softmax over the tokens (rows g and g + 8; columns 2t and 2t + 1)
-      bool grow = false;
-      float x[NT][4];
+      // token 16 u + g + 8 (e >> 1) of the chunk, row 8 j + 2 t + (e & 1)
+      uint32_t hidden = 0;  // bit (u, j, e): the row does not see the key
+      if (edge) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[j][e] = fmaf(sc[j][e], cs[j][e & 1], -m[j][e & 1]);
-          if (edge && key0 + g + 8 * (e >> 1) > pos[j][e & 1]) x[j][e] = -INFINITY;
-          grow |= x[j][e] > kSlack;
-        }
-      if (__any_sync(0xffffffffu, grow)) {
+          for (int e = 0; e < 4; ++e) {
+            const int behind = key0 + g + 8 * (e >> 1) - row_pos[8 * j + 2 * t + (e & 1)];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) hidden |= static_cast<uint32_t>(behind + 16 * u > 0) << ((u * NT + j) * 4 + e);
+          }
+      }
+      float x[SUB][NT][4];
+      float far = -FLT_MAX;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[u][j][e] = fmaf(sc[u][j][e], cs[j][e & 1], -m[j][e & 1]);
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (hidden >> ((u * NT + j) * 4 + e) & 1) x[u][j][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) far = fmaxf(far, x[u][j][e]);
+      if (__any_sync(0xffffffffu, far > kSlack)) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -458,8 +552,10 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
             // the scores themselves: x holds their distance from m, which is no help while m is -FLT_MAX
             float mx = -FLT_MAX;
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
-              if (!(edge && key0 + g + 8 * hf > pos[j][e])) mx = fmaxf(mx, sc[j][e + 2 * hf] * cs[j][e]);
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf)
+                if (!(hidden >> ((u * NT + j) * 4 + e + 2 * hf) & 1)) mx = fmaxf(mx, sc[u][j][e + 2 * hf] * cs[j][e]);
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -474,37 +570,42 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
               o[j][i][2 + e] *= al;
             }
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
-              if (!(edge && key0 + g + 8 * hf > pos[j][e])) x[j][e + 2 * hf] = fmaf(sc[j][e + 2 * hf], cs[j][e], -to);
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf)
+                if (!(hidden >> ((u * NT + j) * 4 + e + 2 * hf) & 1))
+                  x[u][j][e + 2 * hf] = fmaf(sc[u][j][e + 2 * hf], cs[j][e], -to);
           }
       }
-      uint32_t pb[NT][2];
+      uint32_t pb[SUB][NT][2];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        float pr[4];
+      for (int u = 0; u < SUB; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pr[e] = ex2(x[j][e]);
-        l[j][0] += pr[0] + pr[2];
-        l[j][1] += pr[1] + pr[3];
-        pb[j][0] = transpose8x8(pack_f16(pr[0], pr[1]));
-        pb[j][1] = transpose8x8(pack_f16(pr[2], pr[3]));
-      }
+        for (int j = 0; j < NT; ++j) {
+          float pr[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pr[e] = ex2(x[u][j][e]);
+          l[j][0] += pr[0] + pr[2];
+          l[j][1] += pr[1] + pr[3];
+          pb[u][j][0] = transpose8x8(pack_f16(pr[0], pr[1]));
+          pb[u][j][1] = transpose8x8(pack_f16(pr[2], pr[3]));
+        }
       // -------- O^T += V^T P^T
-      {
-        const uint8_t* vs = st + G::CODES;
-        uint32_t vw[4][VB / 4];
-        uint32_t vsc[2][D / 128 + (D == 64)];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        uint32_t vw[4][VW];
+        uint32_t vsc[2][D == 256 ? 2 : 1];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
-          const int r = 2 * t + (i & 1) + 8 * (i >> 1);
-          if constexpr (D == 64) vw[i][0] = *reinterpret_cast<const uint32_t*>(vs + value_at<D>(r, g >> 2) + (g & 3) * 4);
+          const uint8_t* vpt = st + (i & 1 ? voff1 : voff0) + (16 * u + 8 * (i >> 1)) * G::ROW;
+          if constexpr (D == 64) vw[i][0] = *reinterpret_cast<const uint32_t*>(vpt);
           if constexpr (D == 128) {
-            const uint2 v = *reinterpret_cast<const uint2*>(vs + value_at<D>(r, g >> 1) + (g & 1) * 8);
+            const uint2 v = *reinterpret_cast<const uint2*>(vpt);
             vw[i][0] = v.x;
             vw[i][1] = v.y;
           }
           if constexpr (D == 256) {
-            const uint4 v = *reinterpret_cast<const uint4*>(vs + value_at<D>(r, g));
+            const uint4 v = *reinterpret_cast<const uint4*>(vpt);
             vw[i][0] = v.x;
             vw[i][1] = v.y;
             vw[i][2] = v.z;
@@ -513,24 +614,19 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
         }
 #pragma unroll
         for (int pr = 0; pr < 2; ++pr) {
-          const int r = 2 * t + 8 * pr;
-          const uint8_t* sp = st + 2 * G::CODES + G::SCALES + r * G::SROW;
+          const int r = 16 * u + 8 * pr;
+          const uint8_t* sp = st + vsoff + r * G::SROW;
           uint32_t a, b;
-          if constexpr (D == 64) {
-            a = sp[g >> 1];
-            b = sp[G::SROW + (g >> 1)];
-          }
-          if constexpr (D == 128) {
-            a = sp[g];
-            b = sp[G::SROW + g];
-          }
           if constexpr (D == 256) {
-            a = *reinterpret_cast<const uint16_t*>(sp + 2 * g);
-            b = *reinterpret_cast<const uint16_t*>(sp + G::SROW + 2 * g);
+            a = *reinterpret_cast<const uint16_t*>(sp);
+            b = *reinterpret_cast<const uint16_t*>(sp + G::SROW);
+          } else {
+            a = sp[0];
+            b = sp[G::SROW];
           }
           if (edge) {  // a token that no sequence owns: its codes are finite, its scale may be anything
-            if (key0 + r >= s.kv_end) a = 0;
-            if (key0 + r + 1 >= s.kv_end) b = 0;
+            if (key0 + r + 2 * t >= s.kv_end) a = 0;
+            if (key0 + r + 2 * t + 1 >= s.kv_end) b = 0;
           }
           if constexpr (D == 256) {
             vsc[pr][0] = e4m3x2(__byte_perm(a, b, 0x0040));
@@ -540,7 +636,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
           }
         }
 #pragma unroll
-        for (int w = 0; w < VB / 4; ++w) {  // 8 dimensions: four M tiles
+        for (int w = 0; w < VW; ++w) {  // 8 dimensions: four M tiles
           uint32_t ev[2][4], od[2][4];
 #pragma unroll
           for (int pr = 0; pr < 2; ++pr) {
@@ -553,14 +649,18 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
             const uint32_t s0 = vsc[0][D == 256 ? w / 2 : 0], s1 = vsc[1][D == 256 ? w / 2 : 0];
             const uint32_t a[4] = {hmul2(ev[0][i], s0), hmul2(od[0][i], s0), hmul2(ev[1][i], s1), hmul2(od[1][i], s1)};
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma(o[j][4 * w + i], a, pb[j][0], pb[j][1]);
+            for (int j = 0; j < NT; ++j) mma(o[j][4 * w + i], a, pb[u][j][0], pb[u][j][1]);
           }
         }
       }
     }
 
     // -------------------------------------------------------------- the warps' states become one
-    const bool whole = s.pg0 == 0 && s.pg1 == s.pages;
+    if constexpr (K::SHARED) {  // no copy may land in the merge area
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncthreads();
+    }
+    const bool whole = s.whole;
     const int slot = 2 * blockIdx.x + (s.pg0 > 0 ? 0 : 1);
     float* part = p.part_o + static_cast<int64_t>(slot) * ROWS * (D + 2);
 #pragma unroll
@@ -588,7 +688,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
       }
       __syncthreads();
       constexpr int DT = D / 32;  // dimensions of a thread: warp w holds row w of the tile
-      const int row = 8 * j + warp;
+      const int row = 8 * j + (warp & 7);
       float top = -FLT_MAX, sum = 0.f, acc[DT];
 #pragma unroll
       for (int i = 0; i < DT; ++i) acc[i] = 0.f;
@@ -598,11 +698,11 @@ __global__ void __launch_bounds__(THREADS, (Cfg<D, NT>::CTAS)) attn_fp4_kernel(A
       for (int w = 0; w < WARPS; ++w) {
         const float wt = ex2(merge_m[w * ROWS + row] - top);
         sum += wt * merge_l[w * ROWS + row];
-        const float* src = merge_o + (w * 8 + warp) * K::MSTRIDE + lane * DT;
+        const float* src = merge_o + (w * 8 + (warp & 7)) * K::MSTRIDE + lane * DT;
 #pragma unroll
         for (int i = 0; i < DT; ++i) acc[i] += wt * src[i];
       }
-      if (row < s.rows) {
+      if (row < s.rows && warp < 8) {
         if (whole) {
           const float inv = sum == 0.f ? 0.f : p.v_scale / sum;  // no key at all: 0 (a NaN stays one)
           const int rr = s.row0 + row;
@@ -690,7 +790,7 @@ int num_sms() {
 template <int D, int NT>
 int launch(const AttnFp4Params& p, cudaStream_t st) {
   using K = Cfg<D, NT>;
-  static_assert(K::CTAS * (K::SMEM + 1200) <= 227 * 1024, "shared-memory budget");
+  static_assert(K::CTAS * (K::SMEM + 1300) <= 228 * 1024 && K::SMEM <= 226 * 1024, "shared-memory budget");
   static bool ready[kMaxDevices] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -5;
@@ -702,7 +802,7 @@ int launch(const AttnFp4Params& p, cudaStream_t st) {
   }
   const int ctas = K::CTAS * num_sms();
   if (ctas <= 0) return -5;
-  const cudaError_t e = shk::launch(k, dim3(ctas), dim3(THREADS), K::SMEM, st, p);
+  const cudaError_t e = shk::launch(k, dim3(ctas), dim3(K::THREADS), K::SMEM, st, p);
   return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
 }
 }  // namespace
