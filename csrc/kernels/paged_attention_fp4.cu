@@ -42,7 +42,7 @@ namespace attn4 {
 
 constexpr int PAGE = 64;  // tokens of a page
 constexpr float kSlack = 8.f;
-constexpr int kMinPages = 2;  // shortest run
+constexpr int kTable = 16;     // requests of a run that are kept in shared memory
 
 template <int D>
 struct Geo {
@@ -52,14 +52,16 @@ struct Geo {
   static constexpr int PIECES = ROW / 16;        // 16-byte pieces of a token's codes
 };
 // Warps of a CTA, CTAs of an SM, 16-token groups of a warp step (a chunk) and ring stages.  O^T takes D / 4 registers a
-// thread for every 8 rows: one row tile of 8 leaves room for two CTAs of 8 warps (128 registers a thread), more for one
-// CTA of 12 (168) or 8 warps (255).
+// thread for every 8 rows: with 32 of them a thread fits 128 registers and an SM 16 warps, beyond that 8 (255).  At
+// head_dim 128 those 16 are four CTAs, whose starts, merges and ends fall under one another's streaming (decode
+// 64 x 2048: 42 us against 48 with two CTAs of 8); at 64 two are better (64 x 4096: 20 us against 23).
 template <int D, int NT>
 struct Cfg {
   static constexpr int REGS_O = D / 4 * NT;
-  static constexpr int SUB = NT == 1 ? 2 : 1;
-  static constexpr int CTAS = REGS_O <= 32 ? 2 : 1;
-  static constexpr int WARPS = REGS_O <= 32 ? 8 : (REGS_O <= 96 ? 12 : 8);
+  static constexpr int SUB = REGS_O <= 96 && NT <= 3 ? 2 : 1;
+  static constexpr bool QUADS = D == 128 && NT == 1;
+  static constexpr int CTAS = QUADS ? 4 : (REGS_O <= 32 ? 2 : 1);
+  static constexpr int WARPS = QUADS ? 4 : 8;
   static constexpr int THREADS = WARPS * 32;
   static constexpr int CHUNK = 16 * SUB;
   static constexpr int CODES = CHUNK * Geo<D>::ROW;
@@ -67,9 +69,9 @@ struct Cfg {
   static constexpr int STAGE = 2 * (CODES + SCALES);
   static constexpr int MSTRIDE = D + 4;  // floats of a merge row
   static constexpr int MERGE = WARPS * 8 * MSTRIDE * 4;
-  static constexpr int QUERY = NT * D * 16;  // the row tile's fragments
-  static constexpr int STATS = 2 * WARPS * 8 * NT * 4 + 2 * 8 * NT * 4;
-  static constexpr int ROOM = 225 * 1024 / CTAS - QUERY - STATS;
+  static constexpr int QUERY = 2 * NT * D * 16;  // the fragments of two row tiles, this unit's and the next one's
+  static constexpr int STATS = 2 * WARPS * 8 * NT * 4 + 2 * 2 * 8 * NT * 4;
+  static constexpr int ROOM = (227 - 2 * CTAS) * 1024 / CTAS - QUERY - STATS;
   // with two stages that leave no room for the merge area, it takes the ring's place after each unit
   static constexpr bool SHARED = 2 * WARPS * STAGE + MERGE > ROOM;
   static constexpr int FIT = (SHARED ? ROOM : ROOM - MERGE) / (WARPS * STAGE);
@@ -77,6 +79,8 @@ struct Cfg {
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int SMEM = (SHARED ? (RING > MERGE ? RING : MERGE) : RING + MERGE) + QUERY + STATS;
   static_assert(STAGES >= 2, "a chunk in flight while another is used");
+  // shortest run of pages: four chunks a warp (two for one of these runs are no faster, a split costs 3 us)
+  static constexpr int MIN_PAGES = 4 * WARPS * CHUNK / PAGE;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
@@ -180,6 +184,12 @@ __device__ __forceinline__ int64_t weight(const AttnFp4Params& p, const Request&
   return static_cast<int64_t>(r.tiles) * p.hk * r.pages;
 }
 
+// a / b of non-negative numbers, short where both are short.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
 // One unit's part in a CTA's run.
 struct Segment {
   int64_t u0, u1;  // the unit's place among all pages
@@ -196,15 +206,15 @@ struct Cursor {
   Request r;
 };
 template <int ROWS, int CHUNK>
-__device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, Segment& s) {
+__device__ __forceinline__ bool next_segment(const AttnFp4Params& p, const Request* table, int table_b, Cursor& c, Segment& s) {
   const int g = p.hq / p.hk;
   int off = 0;  // pages of the unit that belong to an earlier run
   if (c.tile < 0) {
     if (c.pos >= c.end) return false;
-    const int64_t unit = (c.pos - c.base) / c.r.pages;
-    off = static_cast<int>((c.pos - c.base) % c.r.pages);
-    c.tile = static_cast<int>(unit / p.hk);
-    c.h = static_cast<int>(unit % p.hk);
+    const int64_t unit = quotient(c.pos - c.base, c.r.pages);
+    off = static_cast<int>(c.pos - c.base - unit * c.r.pages);
+    c.tile = static_cast<int>(quotient(unit, p.hk));
+    c.h = static_cast<int>(unit - static_cast<int64_t>(c.tile) * p.hk);
     if (p.whole_units && off) {  // it belongs to the run that it begins in
       c.pos += c.r.pages - off;
       off = 0;
@@ -219,7 +229,8 @@ __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, 
     ++c.tile;
   }
   while (c.tile >= c.r.tiles) {
-    c.r = request(p, ++c.b, ROWS);
+    ++c.b;
+    c.r = c.b - table_b < kTable ? table[c.b - table_b] : request(p, c.b, ROWS);
     c.tile = 0;
   }
   s.b = c.b;
@@ -256,15 +267,17 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   constexpr int VW = D / 64;  // words of a value in a thread (D/8 codes), four M tiles each
   extern __shared__ __align__(128) uint8_t smem[];
   float* merge_o = reinterpret_cast<float*>(smem + (K::SHARED ? 0 : K::RING));
-  uint4* query = reinterpret_cast<uint4*>(smem + K::SMEM - K::STATS - K::QUERY);  // [NT][KW][32 lanes]
+  uint4* query2 = reinterpret_cast<uint4*>(smem + K::SMEM - K::STATS - K::QUERY);  // [2][NT][KW][32 lanes]
   float* merge_m = reinterpret_cast<float*>(smem + K::SMEM - K::STATS);           // [WARPS][ROWS]
   float* merge_l = merge_m + WARPS * ROWS;
-  float* row_scale = merge_l + WARPS * ROWS;           // [ROWS]
-  int* row_pos = reinterpret_cast<int*>(row_scale + ROWS);  // [ROWS] last key a row sees
-  __shared__ int64_t scan[WARPS];
+  float* row_scale2 = merge_l + WARPS * ROWS;                      // [2][ROWS]
+  int* row_pos2 = reinterpret_cast<int*>(row_scale2 + 2 * ROWS);  // [2][ROWS] last key a row sees
+  __shared__ int64_t scan[WARPS + 1];
   __shared__ int64_t start_base;
   __shared__ int start_b;
-  __shared__ int last_flag;
+  __shared__ Request table[kTable];  // of requests start_b, start_b + 1, ...
+  __shared__ Segment open[2];  // units that this CTA has a partial of: at most the run's first and last
+  __shared__ int last_flag[2];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -273,25 +286,15 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   shk::pdl_wait();  // lengths, tables, queries and the new tokens' rows come from earlier kernels
 
   // ---------------------------------------------------------------- this CTA's run
-  int64_t total = 0;
-  for (int b = threadIdx.x; b < p.B; b += THREADS) total += weight(p, request(p, b, ROWS));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) scan[warp] = total;
-  __syncthreads();
-  total = 0;
-  for (int w = 0; w < WARPS; ++w) total += scan[w];
-  __syncthreads();
-  int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  if (per < kMinPages) per = kMinPages;
-  Cursor cons;
-  cons.pos = per * blockIdx.x;
-  cons.end = cons.pos + per;
-  if (cons.end > total) cons.end = total;
-  if (cons.pos >= cons.end) return;
-  for (int64_t done = 0, b0 = 0; b0 < p.B; b0 += THREADS) {
-    const int b = static_cast<int>(b0) + threadIdx.x;
-    const int64_t w = b < p.B ? weight(p, request(p, b, ROWS)) : 0;
+  // The first THREADS requests' pages are summed and searched in one pass, which is all for most batches.
+  int64_t first_w = 0, rest = 0;
+  Request mine = {};
+  if (threadIdx.x < p.B) {
+    mine = request(p, threadIdx.x, ROWS);
+    first_w = weight(p, mine);
+  }
+  for (int b = threadIdx.x + THREADS; b < p.B; b += THREADS) rest += weight(p, request(p, b, ROWS));
+  auto scan_warps = [&](int64_t w) {  // inclusive over the block; the block's sum goes to scan[WARPS]
     int64_t incl = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -300,56 +303,88 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    int64_t before = done;
-    for (int i = 0; i < warp; ++i) before += scan[i];
-    const int64_t hi = before + incl, lo = hi - w;
-    if (lo <= cons.pos && cons.pos < hi) {
-      start_b = b;
-      start_base = lo;
+    int64_t before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      before += i < warp ? scan[i] : 0;
+      all += scan[i];
     }
-    for (int i = 0; i < WARPS; ++i) done += scan[i];
     __syncthreads();
-    if (done > cons.pos) break;
+    if (threadIdx.x == 0) scan[WARPS] = all;
+    return before + incl;
+  };
+  int64_t total = 0;
+  if (p.B > THREADS) {
+    (void)scan_warps(rest);
+    __syncthreads();
+    total = scan[WARPS];
   }
+  int64_t incl = scan_warps(first_w);
+  __syncthreads();
+  int64_t done = scan[WARPS];
+  total += done;
+  int64_t per = quotient(total + gridDim.x - 1, gridDim.x);
+  if (per < K::MIN_PAGES) per = K::MIN_PAGES;
+  Cursor cons;
+  cons.pos = per * blockIdx.x;
+  cons.end = cons.pos + per;
+  if (cons.end > total) cons.end = total;
+  if (cons.pos >= cons.end) return;
+  if (incl - first_w <= cons.pos && cons.pos < incl) {
+    start_b = threadIdx.x;
+    start_base = incl - first_w;
+  }
+  for (int64_t b0 = THREADS; done <= cons.pos; b0 += THREADS) {
+    const int64_t b = b0 + threadIdx.x;
+    const int64_t w = b < p.B ? weight(p, request(p, static_cast<int>(b), ROWS)) : 0;
+    incl = done + scan_warps(w);
+    if (incl - w <= cons.pos && cons.pos < incl) {
+      start_b = static_cast<int>(b);
+      start_base = incl - w;
+    }
+    __syncthreads();
+    done += scan[WARPS];
+    __syncthreads();
+  }
+  __syncthreads();
   cons.b = start_b;
   cons.base = start_base;
   cons.tile = -1;
-  cons.r = request(p, cons.b, ROWS);
+  {
+    const int i = static_cast<int>(threadIdx.x) - start_b;  // start_b + i is this thread's request, if it is among the first
+    if (i >= 0 && i < kTable && threadIdx.x < p.B) table[i] = mine;
+    if (start_b + kTable > THREADS && threadIdx.x < kTable && start_b + threadIdx.x >= THREADS && start_b + threadIdx.x < p.B)
+      table[threadIdx.x] = request(p, start_b + threadIdx.x, ROWS);
+  }
+  __syncthreads();
+  cons.r = table[0];
 
   // ---------------------------------------------------------------- loads of this warp's chunks
   const uint32_t ring = smem_addr(smem) + warp * STAGES * K::STAGE;
   // where this lane's pieces of a chunk go: piece i * 32 + lane is row i * 512 / ROW + lane / PIECES
   const uint32_t kdst = ring + key_at<D>(lane / G::PIECES, lane % G::PIECES);
   const uint32_t vdst = ring + K::CODES + value_at<D>(lane / G::PIECES, lane % G::PIECES);
-  Cursor prod = cons;
-  bool pmore = false;
-  int pc = 0, pc1 = 0, page = 0;  // this warp's next chunk, the segment's end, the chunk's cache block
-  const int32_t* table = nullptr;
-  int64_t head = 0;  // the segment's head inside a block
+  // The loads run ahead into the next unit at most.
+  int pc = 0, pc1 = 0, page = 0;  // this warp's next chunk, the unit's end, the chunk's cache block
+  int at = -1, asked = 0;         // the unit whose chunks are being asked for; chunks asked for so far
+  const int32_t* pages = nullptr;
+  int64_t head = 0;  // the unit's head inside a block
   auto look_up = [&]() {
-    page = table[pc / (PAGE / CHUNK)];
+    page = pages[pc / (PAGE / CHUNK)];
     if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) page = 0;
   };
   auto begin = [&](const Segment& sg) {
     pc = sg.c0 + warp;
     pc1 = sg.c1;
-    table = p.block_tables + static_cast<int64_t>(sg.b) * p.bt_stride;
+    pages = p.block_tables + static_cast<int64_t>(sg.b) * p.bt_stride;
     head = static_cast<int64_t>(sg.h) * G::PAGE_BYTES;
-    pmore = pc < pc1;
-    if (pmore) look_up();
+    ++at;
+    if (pc < pc1) look_up();
   };
-  auto settle = [&]() {  // the next segment with a chunk for this warp
-    Segment sg;
-    do {
-      if (!next_segment<ROWS, CHUNK>(p, prod, sg)) {
-        pmore = false;
-        return;
-      }
-    } while (sg.c0 + warp >= sg.c1);
-    begin(sg);
-  };
-  auto fetch = [&](int stage) {
-    if (pmore) {
+  auto fetch = [&]() {  // the next chunk, if there is one
+    if (pc < pc1) {
+      const int stage = asked % STAGES;
+      ++asked;
       const int64_t off = static_cast<int64_t>(page) * p.hk * G::PAGE_BYTES + head;
       const int part = pc % (PAGE / CHUNK);
       const uint32_t kd = kdst + stage * K::STAGE, vd = vdst + stage * K::STAGE;
@@ -364,16 +399,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       if constexpr (N > 16) cp16<256, 256>(sd, sc);
       pc += WARPS;
       if (pc < pc1) look_up();
-      else if constexpr (K::SHARED) pmore = false;
-      else settle();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  if constexpr (!K::SHARED) {
-    settle();
-#pragma unroll
-    for (int st = 0; st < STAGES - 1; ++st) fetch(st);
-  }
   int it = 0;
 
   // per-lane places of the fragments in a chunk: keys g (+ 8, ...), values 2 t and 2 t + 1 (+ 8, ...)
@@ -385,20 +413,25 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   const int vsoff = 2 * K::CODES + K::SCALES + 2 * t * G::SROW + (D == 64 ? g >> 1 : (D == 128 ? g : 2 * g));
 
   // ---------------------------------------------------------------- segments
-  Segment s;
-  while (next_segment<ROWS, CHUNK>(p, cons, s)) {
-    // The row tile's fragments, a warp per 8 rows: lane (g, t) has dimensions [t D/4, (t + 1) D/4) of row g, word u of
-    // its codes against query[j][u][lane].
+  Segment s, sn;
+  int opened = 0, unit = 0;  // partials left and units done so far; unit's parity: its half of query2
+  auto row_of = [&](const Segment& sg, int n) {  // row n's queries, this lane's dimensions
+    const int rr = sg.row0 + n;
+    return reinterpret_cast<const uint4*>(p.q + (sg.qs + rr / group) * p.q_stride +
+                                          static_cast<int64_t>(sg.h * group + rr % group) * D + t * (D / 4));
+  };
+  // The row tile's fragments, a warp per 8 rows: lane (g, t) has dimensions [t D/4, (t + 1) D/4) of row g, word u of its
+  // codes against query2[half][j][u][lane].
+  auto convert = [&](const Segment& sg, int half) {
 #pragma unroll 1
     for (int j = warp; j < NT; j += WARPS) {
-      const int n = 8 * j + g, rr = s.row0 + n;
+      const int n = 8 * j + g;
       uint4 raw[D / 32];
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (s.qs + rr / group) * p.q_stride +
-                                                        static_cast<int64_t>(s.h * group + rr % group) * D + t * (D / 4));
+      const uint4* src = row_of(sg, n);
       uint32_t top = 0;  // largest magnitude's bf16 bits: its exponent is all that is needed
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        raw[i] = n < s.rows ? src[i] : make_uint4(0, 0, 0, 0);
+        raw[i] = n < sg.rows ? src[i] : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
@@ -413,19 +446,32 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
         uint32_t o[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = pack_f16(__uint_as_float(w[k] << 16) * f, __uint_as_float(w[k] & 0xffff0000u) * f);
-        query[(j * KW + i) * 32 + lane] = make_uint4(o[0], o[1], o[2], o[3]);
+        query2[((half * NT + j) * KW + i) * 32 + lane] = make_uint4(o[0], o[1], o[2], o[3]);
       }
       if (t == 0) {
-        row_scale[n] = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * p.scale_log2;
-        row_pos[n] = s.ctx0 + rr / group;
+        row_scale2[half * ROWS + n] = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * p.scale_log2;
+        row_pos2[half * ROWS + n] = sg.ctx0 + (sg.row0 + n) / group;
       }
     }
-    if constexpr (K::SHARED) {
-      begin(s);
-#pragma unroll
-      for (int st = 0; st < STAGES - 1; ++st) fetch((it + st) % STAGES);
-    }
-    __syncthreads();
+  };
+  bool have = next_segment<ROWS, CHUNK>(p, table, start_b, cons, s);
+  if (have) {
+    begin(s);  // the first keys are on their way before the queries are looked at
+    fetch();
+    convert(s, 0);
+  }
+  __syncthreads();
+  for (; have; s = sn, ++unit) {
+    const int turn = unit & 1;
+    const uint4* query = query2 + turn * NT * KW * 32;
+    const float* row_scale = row_scale2 + turn * ROWS;
+    const int* row_pos = row_pos2 + turn * ROWS;
+    have = next_segment<ROWS, CHUNK>(p, table, start_b, cons, sn);
+    if (have && warp < NT && 8 * warp + g < sn.rows)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(row_of(sn, 8 * warp + g)));
+    // what of the ring could not be filled under the unit before
+    if (at < unit) begin(s);
+    while (asked < it + STAGES - 1 && pc < pc1) fetch();
     float cs[NT][2], m[NT][2], l[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -444,9 +490,12 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
 
 #pragma unroll 1
     for (int c = s.c0 + warp; c < s.c1; c += WARPS, ++it) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+      // a group per chunk: with a full ring STAGES - 2 later ones may still be under way
+      if (asked - it < STAGES - 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
       __syncwarp();
-      fetch((it + STAGES - 1) % STAGES);
+      if (!K::SHARED && pc >= pc1 && at == unit && have) begin(sn);
+      fetch();
       const uint8_t* st = smem + warp * STAGES * K::STAGE + (it % STAGES) * K::STAGE;
       const int key0 = c * CHUNK;
       const bool edge = key0 + CHUNK - 1 > safe;
@@ -655,6 +704,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       }
     }
 
+    if (have) convert(sn, turn ^ 1);  // the barriers below stand before its use
     // -------------------------------------------------------------- the warps' states become one
     if constexpr (K::SHARED) {  // no copy may land in the merge area
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -687,22 +737,24 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
           *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[j][i][e], o[j][i][2 + e], o[j][i + 1][e], o[j][i + 1][2 + e]);
       }
       __syncthreads();
-      constexpr int DT = D / 32;  // dimensions of a thread: warp w holds row w of the tile
-      const int row = 8 * j + (warp & 7);
-      float top = -FLT_MAX, sum = 0.f, acc[DT];
+      constexpr int DT = D / 32;  // dimensions of a thread; a warp takes a row at a time
+#pragma unroll 1
+      for (int rt = warp; rt < 8; rt += WARPS) {
+        const int row = 8 * j + rt;
+        if (row >= s.rows) break;
+        float top = -FLT_MAX, sum = 0.f, acc[DT];
 #pragma unroll
-      for (int i = 0; i < DT; ++i) acc[i] = 0.f;
+        for (int i = 0; i < DT; ++i) acc[i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, merge_m[w * ROWS + row]);
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, merge_m[w * ROWS + row]);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float wt = ex2(merge_m[w * ROWS + row] - top);
-        sum += wt * merge_l[w * ROWS + row];
-        const float* src = merge_o + (w * 8 + (warp & 7)) * K::MSTRIDE + lane * DT;
+        for (int w = 0; w < WARPS; ++w) {
+          const float wt = ex2(merge_m[w * ROWS + row] - top);
+          sum += wt * merge_l[w * ROWS + row];
+          const float* src = merge_o + (w * 8 + rt) * K::MSTRIDE + lane * DT;
 #pragma unroll
-        for (int i = 0; i < DT; ++i) acc[i] += wt * src[i];
-      }
-      if (row < s.rows && warp < 8) {
+          for (int i = 0; i < DT; ++i) acc[i] += wt * src[i];
+        }
         if (whole) {
           const float inv = sum == 0.f ? 0.f : p.v_scale / sum;  // no key at all: 0 (a NaN stays one)
           const int rr = s.row0 + row;
@@ -723,52 +775,66 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       __syncthreads();
     }
     if (!whole) {
-      const int first = static_cast<int>(s.u0 / per), last = static_cast<int>((s.u1 - 1) / per);
-      if (threadIdx.x == 0) {
-        __threadfence();
-        const unsigned n = atomicAdd(&p.tickets[first], 1u);
-        last_flag = n == static_cast<unsigned>(last - first);
-        if (last_flag) p.tickets[first] = 0;
-        __threadfence();
-      }
-      __syncthreads();
-      if (last_flag) {
-        constexpr int DT = D / 32;
-        for (int row = warp; row < s.rows; row += WARPS) {
-          float top = -FLT_MAX, sum = 0.f, acc[DT];
-#pragma unroll
-          for (int i = 0; i < DT; ++i) acc[i] = 0.f;
-          auto at = [&](int c) {
-            return p.part_o + static_cast<int64_t>(2 * c + (c == first ? 1 : 0)) * ROWS * (D + 2);
-          };
-          for (int c = first + lane; c <= last; c += 32) top = fmaxf(top, __ldcg(at(c) + ROWS * D + 2 * row));
-#pragma unroll
-          for (int o2 = 16; o2 > 0; o2 >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
-#pragma unroll 4
-          for (int c = first; c <= last; ++c) {
-            const float* src = at(c);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + ROWS * D + 2 * row));
-            const float wt = ex2(ml.x - top);
-            sum += wt * ml.y;
-#pragma unroll
-            for (int i = 0; i < DT; i += 2) {
-              const float2 v = __ldcg(reinterpret_cast<const float2*>(src + row * D + lane * DT + i));
-              acc[i] += wt * v.x;
-              acc[i + 1] += wt * v.y;
-            }
-          }
-          const float inv = sum == 0.f ? 0.f : p.v_scale / sum;  // no key at all: 0 (a NaN stays one)
-          const int rr = s.row0 + row;
-          __nv_bfloat16* dst = p.out + (s.qs + rr / group) * p.out_stride + static_cast<int64_t>(s.h * group + rr % group) * D + lane * DT;
-#pragma unroll
-          for (int i = 0; i < DT; i += 2)
-            *reinterpret_cast<__nv_bfloat162*>(dst + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
-        }
-      }
-      __syncthreads();  // last_flag is rewritten by the next segment
+      if (threadIdx.x == 0) open[opened] = s;
+      ++opened;
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if (opened == 0) return;
+  // ---------------------------------------------------------------- units cut by a run's end: the last CTA merges
+  __syncthreads();
+  if (threadIdx.x < opened) {
+    const Segment& u = open[threadIdx.x];
+    const int64_t first = quotient(u.u0, per), last = quotient(u.u1 - 1, per);
+    __threadfence();
+    const bool mine = atomicAdd(&p.tickets[first], 1u) == static_cast<unsigned>(last - first);
+    if (mine) p.tickets[first] = 0;
+    last_flag[threadIdx.x] = mine;
+    __threadfence();
+  }
+  __syncthreads();
+  for (int i = 0; i < opened; ++i) {
+    if (!last_flag[i]) continue;
+    const Segment u = open[i];
+    const int first = static_cast<int>(quotient(u.u0, per)), last = static_cast<int>(quotient(u.u1 - 1, per));
+    constexpr int DT = D / 32, BATCH = 4;
+    auto at = [&](int c) { return p.part_o + static_cast<int64_t>(2 * c + (c == first ? 1 : 0)) * ROWS * (D + 2); };
+    for (int row = warp; row < u.rows; row += WARPS) {
+      float top = -FLT_MAX, sum = 0.f, acc[DT];
+#pragma unroll
+      for (int k = 0; k < DT; ++k) acc[k] = 0.f;
+      for (int c = first + lane; c <= last; c += 32) top = fmaxf(top, __ldcg(at(c) + ROWS * D + 2 * row));
+#pragma unroll
+      for (int o2 = 16; o2 > 0; o2 >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
+      for (int c0 = first; c0 <= last; c0 += BATCH) {
+        float2 ml[BATCH], v[BATCH][DT / 2];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+          const float* src = at(c0 + b <= last ? c0 + b : last);
+          ml[b] = __ldcg(reinterpret_cast<const float2*>(src + ROWS * D + 2 * row));
+#pragma unroll
+          for (int k = 0; k < DT / 2; ++k) v[b][k] = __ldcg(reinterpret_cast<const float2*>(src + row * D + lane * DT + 2 * k));
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+          if (c0 + b > last) break;
+          const float wt = ex2(ml[b].x - top);
+          sum += wt * ml[b].y;
+#pragma unroll
+          for (int k = 0; k < DT / 2; ++k) {
+            acc[2 * k] += wt * v[b][k].x;
+            acc[2 * k + 1] += wt * v[b][k].y;
+          }
+        }
+      }
+      const float inv = sum == 0.f ? 0.f : p.v_scale / sum;  // no key at all: 0 (a NaN stays one)
+      const int rr = u.row0 + row;
+      __nv_bfloat16* dst = p.out + (u.qs + rr / group) * p.out_stride + static_cast<int64_t>(u.h * group + rr % group) * D + lane * DT;
+#pragma unroll
+      for (int k = 0; k < DT; k += 2)
+        *reinterpret_cast<__nv_bfloat162*>(dst + k) = __floats2bfloat162_rn(acc[k] * inv, acc[k + 1] * inv);
+    }
+  }
 }
 
 }  // namespace attn4
