@@ -18,6 +18,8 @@ namespace kv4 {
 
 constexpr int PAGE = 64;
 constexpr int WRITE_THREADS = 256;
+// Below, 256 threads a token, else 32 (head_dim 128: 768 tokens take 8.2 us against 10.4, 1500 take 15.7 against 12.2).
+constexpr int64_t kFewTokens = 1200;
 
 template <int D>
 struct Geo {
@@ -25,83 +27,139 @@ struct Geo {
   static constexpr int PAGE_BYTES = PAGE * (ROW + SROW);
 };
 
-// One CTA per token; D/16 neighbouring threads hold a head's 16-dimension blocks, and a thread keeps its block
-// through all heads, so its cosines and sines are read once.
+// A block of 16 dimensions as loaded, and its values.
+struct Raw {
+  uint4 a, b;
+};
+__device__ __forceinline__ Raw fetch(const __nv_bfloat16* p) {
+  return {__ldg(reinterpret_cast<const uint4*>(p)), __ldg(reinterpret_cast<const uint4*>(p) + 1)};
+}
+__device__ __forceinline__ void unpack(const Raw& r, float* v) {
+  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+// A block of 16 rotated query dimensions in bf16.
+__device__ __forceinline__ void put_query(__nv_bfloat16* dst, const float* x) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  uint4* d = reinterpret_cast<uint4*>(dst);
+  d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+// A block of 16 key or value dimensions into its page (block blk of token off).
 template <int D>
-__global__ void __launch_bounds__(WRITE_THREADS) write_kernel(KvFp4WriteParams p) {
+__device__ __forceinline__ void put_cached(uint8_t* page, int off, int blk, float* x, float inv) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    x[i] = __fmul_rn(x[i], inv);
+    amax = fmaxf(amax, fabsf(x[i]));
+  }
+  const __nv_fp8_e4m3 sc(fminf(fmaxf(__fdiv_rn(amax, 6.f), 1.f / 512.f), 448.f));
+  const float sf = static_cast<float>(sc);
+  // a true quotient: multiplying by 1/s moves values that lie between two codes off their tie
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = __fdiv_rn(x[i], sf);
+  *reinterpret_cast<uint2*>(page + off * Geo<D>::ROW + blk * 8) = make_uint2(nvq::e2m1x8(x), nvq::e2m1x8(x + 8));
+  page[PAGE * Geo<D>::ROW + off * Geo<D>::SROW + blk] = sc.__x;
+}
+
+// TPT threads a token.  The rotation pairs dimension d < rot/2 with d + rot/2: where rot/2 is a whole number of blocks
+// (WHOLE) a thread takes a block and its partner, reads their cosines and sines once and keeps them through its heads
+// (every TPT / items-th one); the blocks behind rot go as they are.  Otherwise each block fetches its partners singly.
+//
+// Memory bound: 16384 tokens of 32 + 2 x 8 heads of 128 (363 MB) take 86 us, 65% of the copy rate; what is left is the
+// loads in flight, which 121 registers a thread hold to 16 warps an SM (at 80 registers it spills: 96 us; fetching a
+// head ahead takes 139: 165 us).  With 32 threads a token a thread's cosines serve five heads; with 256 a single token's
+// heads are all in flight.
+template <int D, int TPT, bool WHOLE>
+__global__ void __launch_bounds__(WRITE_THREADS, (TPT == 32 && D < 256 ? 2 : 3)) write_kernel(KvFp4WriteParams p) {
   constexpr int BLOCKS = D / 16;
-  constexpr int HEADS = WRITE_THREADS / BLOCKS;  // heads in flight
   shk::pdl_trigger();
   shk::pdl_wait();
-  const int64_t tok = blockIdx.x;
-  const int blk = threadIdx.x % BLOCKS, d0 = blk * 16;
+  const int64_t tok = static_cast<int64_t>(blockIdx.x) * (WRITE_THREADS / TPT) + threadIdx.x / TPT;
+  if (tok >= p.num_tokens) return;
+  const int tid = threadIdx.x % TPT;
   const int half = p.rot / 2;
   int64_t pos = p.positions[tok];
   if (pos < 0 || pos >= p.max_pos) pos = 0;  // never past the table
   const float* cs = p.cos_sin + pos * p.rot;
-  // The rotation of dimension d < rot pairs it with d +- half: x'[d] = x[d] c - x[d + half] s below half, and
-  // x[d] c + x[d - half] s above.
-  float c[16], s[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int d = d0 + i;
-    const int j = d < half ? d : d - half;
-    c[i] = d < p.rot ? cs[j] : 1.f;
-    s[i] = d < p.rot ? (d < half ? -cs[half + j] : cs[half + j]) : 0.f;
-  }
   const int64_t slot = p.slots[tok];
   const bool cached = slot >= 0 && slot < p.num_slots;
-  const int64_t page = slot / PAGE;
+  const int64_t page = cached ? slot / PAGE : 0;
   const int off = static_cast<int>(slot % PAGE);
   const __nv_bfloat16* row = p.qkv + tok * p.qkv_stride;
-  for (int h = threadIdx.x / BLOCKS; h < p.hq + 2 * p.hk; h += HEADS) {
-    if (h >= p.hq && !cached) break;
-    const __nv_bfloat16* hp = row + static_cast<int64_t>(h) * D;
-    float x[16];
-    nvq::load16(hp + d0, x);
-    if (h < p.hq + p.hk && d0 < p.rot) {
-      float y[16];
-      if (half % 16 == 0) {  // the partners are another whole block
-        nvq::load16(hp + (d0 < half ? d0 + half : d0 - half), y);
-      } else {
+  const int heads = cached ? p.hq + p.hk : p.hq;
+  auto put = [&](int h, int blk, float* x) {
+    if (h < p.hq) put_query(p.q_out + tok * p.q_stride + static_cast<int64_t>(h) * D + blk * 16, x);
+    else put_cached<D>(p.k_cache + (page * p.hk + h - p.hq) * Geo<D>::PAGE_BYTES, off, blk, x, p.k_inv);
+  };
+  if constexpr (WHOLE) {
+    const int pairs = half / 16, items = BLOCKS - pairs, step = TPT / items;
+    const int item = tid % items;
+    int h = tid / items;
+    if (h < step) {
+      if (item < pairs) {
+        float c[16], s[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int d = d0 + i;
-          y[i] = d < p.rot ? __bfloat162float(hp[d < half ? d + half : d - half]) : 0.f;
+        for (int i = 0; i < 4; ++i) {
+          *reinterpret_cast<float4*>(c + 4 * i) = reinterpret_cast<const float4*>(cs + item * 16)[i];
+          *reinterpret_cast<float4*>(s + 4 * i) = reinterpret_cast<const float4*>(cs + half + item * 16)[i];
+        }
+        for (; h < heads; h += step) {
+          const __nv_bfloat16* hp = row + static_cast<int64_t>(h) * D + item * 16;
+          const Raw xa = fetch(hp), ya = fetch(hp + half);
+          float x[16], y[16], z[16];
+          unpack(xa, x);
+          unpack(ya, y);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) z[i] = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i]));
+          put(h, item, z);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) z[i] = __fadd_rn(__fmul_rn(y[i], c[i]), __fmul_rn(x[i], s[i]));
+          put(h, item + pairs, z);
+        }
+      } else {
+        for (; h < heads; h += step) {
+          float x[16];
+          unpack(fetch(row + static_cast<int64_t>(h) * D + (item + pairs) * 16), x);
+          put(h, item + pairs, x);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i]));
     }
-    if (h < p.hq) {
-      uint32_t w[8];
+  } else {
+    const int blk = tid % BLOCKS, d0 = blk * 16;
+    for (int h = tid / BLOCKS; h < heads; h += TPT / BLOCKS) {
+      const __nv_bfloat16* hp = row + static_cast<int64_t>(h) * D;
+      float x[16];
+      unpack(fetch(hp + d0), x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+      for (int i = 0; i < 16; ++i) {
+        const int d = d0 + i;
+        if (d >= p.rot) break;
+        const int j = d < half ? d : d - half;
+        const float y = __bfloat162float(hp[d < half ? d + half : j]);
+        const float u = __fmul_rn(x[i], cs[j]), v = __fmul_rn(y, cs[half + j]);
+        x[i] = d < half ? __fsub_rn(u, v) : __fadd_rn(u, v);
       }
-      uint4* dst = reinterpret_cast<uint4*>(p.q_out + tok * p.q_stride + static_cast<int64_t>(h) * D + d0);
-      dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-      continue;
+      put(h, blk, x);
     }
-    const bool key = h < p.hq + p.hk;
-    const int hk = key ? h - p.hq : h - p.hq - p.hk;
-    const float inv = key ? p.k_inv : p.v_inv;
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[i] = __fmul_rn(x[i], inv);
-      amax = fmaxf(amax, fabsf(x[i]));
-    }
-    const __nv_fp8_e4m3 sc(fminf(fmaxf(__fdiv_rn(amax, 6.f), 1.f / 512.f), 448.f));
-    const float sf = static_cast<float>(sc);
-    // a true quotient: multiplying by 1/s moves values that lie between two codes off their tie
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = __fdiv_rn(x[i], sf);
-    uint8_t* pg = (key ? p.k_cache : p.v_cache) + (page * p.hk + hk) * Geo<D>::PAGE_BYTES;
-    *reinterpret_cast<uint2*>(pg + off * Geo<D>::ROW + blk * 8) = make_uint2(nvq::e2m1x8(x), nvq::e2m1x8(x + 8));
-    pg[PAGE * Geo<D>::ROW + off * Geo<D>::SROW + blk] = sc.__x;
+  }
+  if (!cached) return;
+  const int blk = tid % BLOCKS;
+  constexpr int STEP = TPT / BLOCKS;
+  for (int h = tid / BLOCKS; h < p.hk; h += STEP) {
+    float x[16];
+    unpack(fetch(row + static_cast<int64_t>(p.hq + p.hk + h) * D + blk * 16), x);
+    put_cached<D>(p.v_cache + (page * p.hk + h) * Geo<D>::PAGE_BYTES, off, blk, x, p.v_inv);
   }
 }
 
@@ -179,6 +237,20 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_kernel(const __grid_constan
 
 using namespace shk::kv4;
 
+namespace {
+template <int D, int TPT>
+cudaError_t launch_write(const KvFp4WriteParams& p, cudaStream_t stream) {
+  constexpr int TOKENS = WRITE_THREADS / TPT;
+  const dim3 grid(static_cast<unsigned>((p.num_tokens + TOKENS - 1) / TOKENS)), block(WRITE_THREADS);
+  return p.rot % 32 == 0 ? shk::launch(write_kernel<D, TPT, true>, grid, block, 0, stream, p)
+                         : shk::launch(write_kernel<D, TPT, false>, grid, block, 0, stream, p);
+}
+template <int D>
+cudaError_t launch_write(const KvFp4WriteParams& p, cudaStream_t stream) {
+  return p.num_tokens < kFewTokens ? launch_write<D, 256>(p, stream) : launch_write<D, 32>(p, stream);
+}
+}  // namespace
+
 extern "C" int sh_kv_fp4_write(const KvFp4WriteParams* params, int head_dim, cudaStream_t stream) {
   const KvFp4WriteParams& p = *params;
   if (p.num_tokens <= 0) return 0;
@@ -186,12 +258,11 @@ extern "C" int sh_kv_fp4_write(const KvFp4WriteParams* params, int head_dim, cud
   if ((reinterpret_cast<uintptr_t>(p.qkv) & 15) || (p.qkv_stride & 7) || (reinterpret_cast<uintptr_t>(p.q_out) & 15) ||
       (p.q_stride & 7) || (reinterpret_cast<uintptr_t>(p.k_cache) & 15) || (reinterpret_cast<uintptr_t>(p.v_cache) & 15))
     return -3;
-  const dim3 grid(static_cast<unsigned>(p.num_tokens)), block(WRITE_THREADS);
   cudaError_t e;
   switch (head_dim) {
-    case 64: e = shk::launch(write_kernel<64>, grid, block, 0, stream, p); break;
-    case 128: e = shk::launch(write_kernel<128>, grid, block, 0, stream, p); break;
-    case 256: e = shk::launch(write_kernel<256>, grid, block, 0, stream, p); break;
+    case 64: e = launch_write<64>(p, stream); break;
+    case 128: e = launch_write<128>(p, stream); break;
+    case 256: e = launch_write<256>(p, stream); break;
     default: return -4;
   }
   return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
