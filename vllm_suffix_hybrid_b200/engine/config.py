@@ -64,7 +64,7 @@ class ModelConfig:
     dsa_topk: int = 0
     # --- quantisation ---
     weight_format: str = "bf16"  # bf16 | fp8_block | nvfp4
-    kv_format: str = "bf16"  # bf16 | fp8 | nvfp4
+    kv_format: str = "bf16"  # bf16 | fp8 | nvfp4 (GQA: bf16 | nvfp4; SUFFIX_HYBRID_KV_FORMAT)
     # --- draft head ---
     draft: str = "eagle"  # eagle | mtp | none
     draft_layers: int = 1
@@ -257,6 +257,8 @@ def apply_env(cfg: EngineConfig) -> EngineConfig:
         cfg.chunked_prefill = _env("CHUNKED_PREFILL") == "1"
     if _env("HOST_KV") == "1":
         cfg.cache.host_kv = True
+    if _env("KV_FORMAT") in ("bf16", "nvfp4"):
+        cfg.model.kv_format = _env("KV_FORMAT")
     v = _env("HOST_KV_HOT_ROWS")
     if v is not None and v.isdigit():
         cfg.cache.host_kv_hot_rows = int(v)

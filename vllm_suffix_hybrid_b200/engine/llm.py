@@ -33,7 +33,7 @@ from typing import Dict, List, Optional
 import numpy as np
 import torch
 
-from .. import _native
+from .. import _native, ops
 from ..models import build_model
 from ..parallel import state as pstate
 from .config import EngineConfig, apply_env
@@ -148,14 +148,15 @@ class LLMEngine:
             self.caches = self.model.allocate_caches(num_blocks, bs, cfg.max_num_seqs + 1, self.k + 1)
             self.host_tier = getattr(self.model, "host_tier", None)
         else:
-            self.caches = allocate_caches(mcfg.layers, self.model.kv_cache_shape(num_blocks, bs), self.model.dtype,
-                                          dev)
+            self.caches = allocate_caches(mcfg.layers, self.model.kv_cache_shape(num_blocks, bs),
+                                          self.model.kv_cache_dtype, dev)
         if self.draft is None:
             self.dcaches = None
         elif hasattr(self.draft, "allocate_caches"):
             self.dcaches = self.draft.allocate_caches(num_blocks, bs)
         else:
-            self.dcaches = allocate_caches(1, self.model.kv_cache_shape(num_blocks, bs), self.model.dtype, dev)[0]
+            self.dcaches = allocate_caches(1, self.model.kv_cache_shape(num_blocks, bs), self.model.kv_cache_dtype,
+                                           dev)[0]
         self._free_slots = list(range(cfg.max_num_seqs, 0, -1))
         self.runner = Runner(self.model, self.draft, self.caches, self.dcaches, self.k, cfg.max_num_seqs,
                              self.max_blocks_per_seq, bs, dev, cfg.cuda_graphs)
@@ -222,7 +223,7 @@ class LLMEngine:
         free, _ = torch.cuda.mem_get_info()
         m = self.model
         kv_layers = getattr(m, "num_kv_layers", c.model.layers)
-        if hasattr(m, "kv_block_bytes"):  # latent-cache models size their own rows (MLA: NVFP4 or bf16 + indexer)
+        if hasattr(m, "kv_block_bytes"):  # models size their own rows (GQA: bf16 or NVFP4; MLA: latent + indexer)
             per_block = m.kv_block_bytes(self.block_size) * kv_layers
             if self.draft is not None:
                 per_block += (self.draft.kv_block_bytes(self.block_size) if hasattr(self.draft, "kv_block_bytes")
@@ -286,6 +287,74 @@ class LLMEngine:
         self._propose(batch_native=True)
         return rids
 
+    def fork_request(self, rid: str, tokens=(), max_new_tokens: int = 128, new_rid: Optional[str] = None,
+                     stop_token_ids=None) -> str:
+        """A new request that continues a running one from where it stands, with `tokens` behind its history.
+
+        The prompt is the parent's history plus tokens.  The parent's full cache blocks are shared, its last,
+        partly filled one is copied in every layer (the two requests write different tokens there), so only the
+        tokens behind the parent's cache are prefilled.  Attention-only models; both requests go on independently
+        and may be forked again."""
+        if self.runner.recurrent or self.dp > 1 or self.host_tier is not None:
+            raise ValueError("fork_request needs an attention-only model on one data-parallel rank, without the host "
+                             "KV tier")
+        self._drain()
+        parent = next((r for r in self.running if r.rid == rid and not r.finished), None)
+        if parent is None:
+            raise ValueError(f"request {rid} is not running")
+        prompt = np.concatenate([parent.prompt, np.asarray(parent.output, dtype=np.int64),
+                                 np.asarray(tokens, dtype=np.int64)])
+        full, part = divmod(parent.committed, self.block_size)
+        if part and not self._unclaimed_blocks():
+            raise MemoryError("no unpromised KV block for the fork's copy of the parent's last block")
+        new_rid = self.add_request(prompt, max_new_tokens, new_rid, stop_token_ids)
+        r = self.waiting[-1]
+        shared = parent.blocks[:full]
+        self.pool.share(shared)
+        r.blocks = list(shared)
+        if part:
+            own = self.pool.allocate(1)
+            ids = torch.tensor([parent.blocks[full], own[0]], device=self.device)
+            ops.copy_kv_pages(self._block_tensors(), ids[:1], ids[1:])
+            r.blocks += own
+        r.prefilled = parent.committed
+        return new_rid
+
+    def compact_cache(self) -> int:
+        """Moves the held cache blocks to the lowest ids, in every layer; returns how many there are (block 0, the
+        scratch block, not counted): the caches' first that many + 1 blocks then hold every request's keys and
+        values, for a snapshot or to take the rest back."""
+        if self.host_tier is not None:
+            raise ValueError("compact_cache does not move host-tier rows")
+        self._drain()
+        moves = self.pool.compaction()
+        if moves:
+            ops.copy_kv_pages(self._block_tensors(), torch.tensor(list(moves), device=self.device),
+                              torch.tensor(list(moves.values()), device=self.device))
+            for r in self.running + self.waiting + ([self.prefilling] if self.prefilling is not None else []):
+                r.blocks = [moves.get(b, b) for b in r.blocks]
+                r.blocks_np = np.asarray(r.blocks, dtype=np.int32)
+            self.pool.moved(moves)
+        return self.pool.num_blocks - 1 - self.pool.free
+
+    def _block_tensors(self) -> List[torch.Tensor]:
+        """Every cache tensor that is laid out by blocks (recurrent states are not)."""
+        out = []
+
+        def walk(x):
+            if isinstance(x, torch.Tensor):
+                out.append(x)
+            elif isinstance(x, dict):
+                for v in x.values():
+                    walk(v)
+            elif isinstance(x, (list, tuple)):
+                for v in x:
+                    walk(v)
+
+        walk(self.caches)
+        walk(self.dcaches)
+        return [t for t in out if t.dim() > 1 and t.shape[0] == self.pool.num_blocks]
+
     def _fill_caches_random(self, seed: int) -> None:
         gen = torch.Generator(device=self.device).manual_seed(seed) if torch.device(self.device).type == "cuda" \
             else torch.Generator().manual_seed(seed)
@@ -333,6 +402,8 @@ class LLMEngine:
         for i, r in enumerate(self.waiting):
             if r.rid == rid:
                 self.waiting.pop(i)
+                self.pool.release(r.blocks)  # a fork's shared blocks
+                r.blocks = []
                 r.finished, r.finish_reason = True, "abort"
                 self.finished[rid] = r
                 return True
@@ -475,11 +546,11 @@ class LLMEngine:
         # a waiting request is prefilled once a row is free and the KV blocks not promised to running requests
         # cover it (otherwise the running ones decode on, without breaking the decode pipeline, until they do)
         if self.waiting and free_rows > 0 and (not self.running or
-                                               self._reservation(self.waiting[0]) <= self._unclaimed_blocks()):
+                                               self._missing(self.waiting[0]) <= self._unclaimed_blocks()):
             if self._chunkable(self.waiting[0]):
                 r0 = self.waiting[0]
-                if not self.running and self._reservation(r0) > self._unclaimed_blocks():
-                    raise MemoryError(f"request {r0.rid} needs {self._reservation(r0)} KV blocks, the pool has "
+                if not self.running and self._missing(r0) > self._unclaimed_blocks():
+                    raise MemoryError(f"request {r0.rid} needs {self._missing(r0)} KV blocks, the pool has "
                                       f"{self.pool.free} free")
                 if self.prefilling is None:
                     self._drain()
@@ -530,18 +601,22 @@ class LLMEngine:
         look-ahead (the decode step keeps blocks for committed + 2k + 2 positions)."""
         return blocks_for(len(r.prompt) + r.max_new_tokens + 2 * self.k + 2, self.block_size)
 
+    def _missing(self, r: Request) -> int:
+        """Blocks of the reservation that r does not hold yet (a fork starts with some)."""
+        return max(0, self._reservation(r) - len(r.blocks))
+
     def _unclaimed_blocks(self) -> int:
         """Free blocks not yet promised to a running request's remaining growth."""
-        owed = sum(max(0, self._reservation(r) - len(r.blocks)) for r in self.running)
+        owed = sum(self._missing(r) for r in self.running)
         if self.prefilling is not None:
-            owed += max(0, self._reservation(self.prefilling) - len(self.prefilling.blocks))
+            owed += self._missing(self.prefilling)
         return self.pool.free - owed
 
     def _chunkable(self, r: Request) -> bool:
         """Whether r's prompt is prefilled in chunks (longer than the prefill budget, attention-only model,
-        no data-parallel lockstep)."""
-        return (self.cfg.chunked_prefill and len(r.prompt) > self.cfg.max_prefill_tokens and self.dp == 1
-                and not self.runner.recurrent)
+        no data-parallel lockstep); a fork's always is, from the end of what it shares."""
+        return r.prefilled > 0 or (self.cfg.chunked_prefill and len(r.prompt) > self.cfg.max_prefill_tokens
+                                   and self.dp == 1 and not self.runner.recurrent)
 
     def _chunk_step(self) -> StepStats:
         """Prefill the next max_prefill_tokens of the long prompt; its last chunk makes it a running request."""
@@ -583,7 +658,7 @@ class LLMEngine:
         blocks = self._unclaimed_blocks()
         while self.waiting and len(batch) < free_rows:
             r = self.waiting[0]
-            if batch and len(r.prompt) > budget:
+            if r.prefilled or (batch and len(r.prompt) > budget):
                 break
             need = self._reservation(r)
             if need > blocks:

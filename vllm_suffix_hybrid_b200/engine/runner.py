@@ -213,7 +213,7 @@ class Runner:
         nsplit = ops.attention_splits(tr.numel(), kvh, self.max_blocks)
         return AttnMeta(positions=pos.reshape(-1), slot_mapping=self._slots(bt, pos).reshape(-1), block_tables=bt,
                         seq_lens=seq_lens, q_start=qs, tile_req=tr, tile_row0=t0, num_tokens=nb * qlen,
-                        nsplit=nsplit, max_rows=_max_rows(qlen * self.group))
+                        nsplit=nsplit, max_rows=_max_rows(qlen * self.group), max_q=qlen)
 
     def _draft_steps(self, d1: torch.Tensor, f1: torch.Tensor, lnew: torch.Tensor, bt: torch.Tensor, nb: int):
         """Draft tokens 2..k at positions lnew + s - 2 (s = 2..k)."""
@@ -367,7 +367,7 @@ class Runner:
                         tile_req=torch.tensor(tr, dtype=torch.int32, device=dev),
                         tile_row0=torch.tensor(t0, dtype=torch.int32, device=dev), num_tokens=int(sum(lens)),
                         nsplit=ops.attention_splits(len(tr), self.model.kv_heads_local, mb),
-                        max_rows=_max_rows(max(lens) * self.group))
+                        max_rows=_max_rows(max(lens) * self.group), max_q=max(lens))
         slot_t = torch.tensor(state_slots if state_slots is not None else [0] * n, dtype=torch.long, device=dev)
         meta.state_slots, meta.pending, meta.window = slot_t, self.pending, 0
         hid, pre = self.model.forward(ids, meta, self.caches)

@@ -36,6 +36,7 @@ class AttnMeta:
     num_tokens: int = 0
     nsplit: int = 1  # KV splits per request (split-KV attention)
     max_rows: int = 64  # most valid rows in any 64-row query tile
+    max_q: int = 1  # most new tokens of any request (4-bit cache attention)
     state_slots: Optional[torch.Tensor] = None  # [B] int64 recurrent-state slot per request
     pending: Optional[torch.Tensor] = None  # [slots] int32 accepted window records to replay
     window: int = 0  # verify-window length (0: prefill from an empty state)
@@ -118,6 +119,45 @@ class RMSNorm:
         return ops.rms_norm(x, self.weight, self.eps)
 
 
+def fp4_kv(cfg, block_size: int = 64) -> bool:
+    """Whether a GQA model's paged cache is 4-bit (kv_format "nvfp4"); refuses shapes it does not have."""
+    if cfg.kv_format != "nvfp4":
+        return False
+    if cfg.head_dim not in (64, 128, 256) or block_size != 64:
+        raise ValueError(f"the 4-bit KV cache needs head_dim 64, 128 or 256 and 64-token blocks, got head_dim "
+                         f"{cfg.head_dim} and blocks of {block_size}")
+    return True
+
+
+def gqa_cache(cfg, kv_heads: int, num_blocks: int, block_size: int, dtype):
+    """(shape, dtype) of one layer's key or value cache."""
+    if fp4_kv(cfg, block_size):
+        return ops.kv_fp4_cache_shape(num_blocks, kv_heads, cfg.head_dim), torch.uint8
+    return (num_blocks, kv_heads, block_size, cfg.head_dim), dtype
+
+
+def gqa_block_bytes(cfg, kv_heads: int, block_size: int, dtype) -> int:
+    """Bytes of one block in a layer's two caches."""
+    shape, dt = gqa_cache(cfg, kv_heads, 1, block_size, dtype)
+    return 2 * math.prod(shape) * torch.empty(0, dtype=dt).element_size()
+
+
+def cached_attention(qkv: torch.Tensor, meta: AttnMeta, kv: tuple, cos_sin: torch.Tensor, hq: int, hk: int, d: int,
+                     rot: int, scale: float, kv_scales=(1.0, 1.0)) -> torch.Tensor:
+    """RoPE, the new tokens into the paged cache, attention over it: [T, hq * d].  A uint8 cache holds NVFP4 rows
+    (quantised as they are written; kv_scales divide keys and values before)."""
+    k_cache, v_cache = kv
+    attn = torch.empty(qkv.shape[0], hq * d, dtype=qkv.dtype, device=qkv.device)
+    if k_cache.dtype == torch.uint8:
+        q = ops.rope_kv_write_fp4(qkv, meta.positions, cos_sin, k_cache, v_cache, meta.slot_mapping, hq, hk, d, rot,
+                                  *kv_scales)
+        return ops.paged_attention_fp4(attn, q, k_cache, v_cache, meta.block_tables, meta.seq_lens, meta.q_start, hq, d,
+                                       scale, meta.max_q, *kv_scales)
+    ops.rope_kv_write(qkv, meta.positions, cos_sin, k_cache, v_cache, meta.slot_mapping, hq, hk, d, rot)
+    return ops.paged_attention(attn, qkv, k_cache, v_cache, meta.block_tables, meta.seq_lens, meta.q_start,
+                               meta.tile_req, meta.tile_row0, hq, scale, meta.nsplit, meta.max_rows)
+
+
 class Attention:
     """GQA attention with fused QKV, RoPE + cache write, paged attention, o_proj."""
 
@@ -136,16 +176,11 @@ class Attention:
                           sections=[q_full, kv_full, kv_full])
         self.o = Linear(cfg.heads * cfg.head_dim, h, dtype, device, gen, parallel="row")
         self.cos_sin = cos_sin
+        self.kv_scales = (1.0, 1.0)  # what a 4-bit cache divides keys and values by before their block scales
 
     def __call__(self, x: torch.Tensor, meta: AttnMeta, kv: tuple) -> torch.Tensor:
-        qkv = self.qkv(x)
-        k_cache, v_cache = kv
-        ops.rope_kv_write(qkv, meta.positions, self.cos_sin, k_cache, v_cache, meta.slot_mapping, self.hq, self.hk,
-                          self.d, self.rot)
-        attn = torch.empty(x.shape[0], self.hq * self.d, dtype=x.dtype, device=x.device)
-        ops.paged_attention(attn, qkv, k_cache, v_cache, meta.block_tables, meta.seq_lens, meta.q_start,
-                            meta.tile_req, meta.tile_row0, self.hq, self.scale, meta.nsplit,
-                            meta.max_rows)
+        attn = cached_attention(self.qkv(x), meta, kv, self.cos_sin, self.hq, self.hk, self.d, self.rot, self.scale,
+                                self.kv_scales)
         return self.o(attn)  # partial sum under TP (reduced by the caller)
 
 

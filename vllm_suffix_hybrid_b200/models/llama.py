@@ -12,7 +12,8 @@ import torch
 
 from .. import ops
 from ..parallel import comm, state
-from .common import AttnMeta, DecoderLayer, Linear, RMSNorm, dtype_of, init_weight
+from .common import (AttnMeta, DecoderLayer, Linear, RMSNorm, dtype_of, fp4_kv, gqa_block_bytes, gqa_cache,
+                     init_weight)
 
 
 class LlamaModel:
@@ -38,7 +39,14 @@ class LlamaModel:
         return self.cfg.kv_heads // state.get().tp
 
     def kv_cache_shape(self, num_blocks: int, block_size: int) -> Tuple[int, ...]:
-        return (num_blocks, self.kv_heads_local, block_size, self.cfg.head_dim)
+        return gqa_cache(self.cfg, self.kv_heads_local, num_blocks, block_size, self.dtype)[0]
+
+    @property
+    def kv_cache_dtype(self) -> torch.dtype:
+        return torch.uint8 if fp4_kv(self.cfg) else self.dtype
+
+    def kv_block_bytes(self, block_size: int) -> int:
+        return gqa_block_bytes(self.cfg, self.kv_heads_local, block_size, self.dtype)
 
     # -- forward --------------------------------------------------------------
     def forward(self, ids: torch.Tensor, meta: AttnMeta, kv_caches: List[tuple],

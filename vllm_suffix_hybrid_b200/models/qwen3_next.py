@@ -23,7 +23,7 @@ import torch
 
 from .. import ops
 from ..parallel import comm, state
-from .common import AttnMeta, Linear, RMSNorm, dtype_of, init_weight
+from .common import AttnMeta, Linear, RMSNorm, cached_attention, dtype_of, gqa_block_bytes, gqa_cache, init_weight
 from .moe import MoEBlock
 
 
@@ -99,6 +99,7 @@ class GatedAttention:
         self.k_norm = RMSNorm(cfg.head_dim, cfg.norm_eps, dtype, device)
         self.o = Linear(q, cfg.hidden, dtype, device, gen, parallel="row")
         self.cos_sin = cos_sin
+        self.kv_scales = (1.0, 1.0)  # what a 4-bit cache divides keys and values by before their block scales
 
     def __call__(self, x: torch.Tensor, meta: AttnMeta, kv) -> torch.Tensor:
         T = x.shape[0]
@@ -106,12 +107,7 @@ class GatedAttention:
         qkvg = self.qkvg(x)
         ops.rms_norm_heads(qkvg[:, : hq * d].view(T, hq, d), self.q_norm.weight, self.q_norm.eps)
         ops.rms_norm_heads(qkvg[:, hq * d:(hq + hk) * d].view(T, hk, d), self.k_norm.weight, self.k_norm.eps)
-        k_cache, v_cache = kv
-        ops.rope_kv_write(qkvg, meta.positions, self.cos_sin, k_cache, v_cache, meta.slot_mapping, hq, hk, d,
-                          self.rot)
-        attn = torch.empty(T, hq * d, dtype=x.dtype, device=x.device)
-        ops.paged_attention(attn, qkvg, k_cache, v_cache, meta.block_tables, meta.seq_lens, meta.q_start,
-                            meta.tile_req, meta.tile_row0, hq, self.scale, meta.nsplit, meta.max_rows)
+        attn = cached_attention(qkvg, meta, kv, self.cos_sin, hq, hk, d, self.rot, self.scale, self.kv_scales)
         gate = qkvg[:, (hq + 2 * hk) * d:(2 * hq + 2 * hk) * d]
         attn = (attn.float() * torch.sigmoid(gate.float())).to(x.dtype)
         return self.o(attn)
@@ -160,15 +156,20 @@ class Qwen3NextModel:
         return sum(1 for l in self.layers if l.kind == "A")
 
     def kv_cache_shape(self, num_blocks: int, block_size: int):
-        return (num_blocks, self.kv_heads_local, block_size, self.cfg.head_dim)
+        return gqa_cache(self.cfg, self.kv_heads_local, num_blocks, block_size, self.dtype)[0]
+
+    def kv_block_bytes(self, block_size: int) -> int:
+        return gqa_block_bytes(self.cfg, self.kv_heads_local, block_size, self.dtype)
+
+    def attention_cache(self, num_blocks: int, block_size: int) -> tuple:
+        shape, dt = gqa_cache(self.cfg, self.kv_heads_local, num_blocks, block_size, self.dtype)
+        return torch.zeros(shape, dtype=dt, device=self.device), torch.zeros(shape, dtype=dt, device=self.device)
 
     def allocate_caches(self, num_blocks: int, block_size: int, slots: int, window: int) -> List:
         caches = []
         for l in self.layers:
             if l.kind == "A":
-                shp = self.kv_cache_shape(num_blocks, block_size)
-                caches.append((torch.zeros(shp, dtype=self.dtype, device=self.device),
-                               torch.zeros(shp, dtype=self.dtype, device=self.device)))
+                caches.append(self.attention_cache(num_blocks, block_size))
             else:
                 caches.append(l.mixer.make_cache(slots, window, self.device))
         return caches
@@ -207,9 +208,7 @@ class MtpHead:
         self.norm = RMSNorm(cfg.hidden, cfg.norm_eps, dt, device)
 
     def allocate_caches(self, num_blocks: int, block_size: int):
-        shp = self.target.kv_cache_shape(num_blocks, block_size)
-        return (torch.zeros(shp, dtype=self.target.dtype, device=self.target.device),
-                torch.zeros(shp, dtype=self.target.dtype, device=self.target.device))
+        return self.target.attention_cache(num_blocks, block_size)
 
     def forward(self, tokens, feature, meta: AttnMeta, kv):
         e = self.enorm(ops.embedding(tokens, self.target.embed))
