@@ -5,10 +5,10 @@
 //
 // Work.  A unit is (request, kv head, tile of NT * 8 packed query rows); packed row r of a request is token r / G,
 // head r % G of the group, so the heads of a group and the tokens of a verify window share one read of the keys.
-// The units' pages, laid end to end, are cut into equal runs, one per CTA (2 CTAs an SM for one 8-row tile): a
-// ragged batch loads every SM alike and no length has to be known on the host.  A unit cut by a run's end leaves an
-// fp32 partial (O, max, sum); the last of its CTAs to finish (a ticket, which it resets) merges them in page order,
-// so the result does not depend on the order of arrival.
+// The units, each as long as its pages and a constant for its start and end, are laid end to end and cut into equal
+// runs, one per CTA: a ragged batch loads every SM alike and no length has to be known on the host.  A unit that a run's
+// end leaves in two or more pieces has fp32 partials (O, max, sum); the last of its CTAs to finish (a ticket, which it
+// resets) merges them in page order, so the result does not depend on the order of arrival.
 //
 // A CTA's warps take the run's 32-token chunks in turn, each through a ring of its own in shared memory, filled with
 // cp.async: no barrier between the warps while they stream.  Per chunk and warp, with m16n8k16 (f16 in, fp32 out) and
@@ -42,6 +42,7 @@ namespace attn4 {
 
 constexpr int PAGE = 64;  // tokens of a page
 constexpr float kSlack = 8.f;
+constexpr int kUnit = 8;       // pages' worth of work that a unit costs besides its pages
 constexpr int kTable = 16;     // requests of a run that are kept in shared memory
 
 template <int D>
@@ -79,8 +80,8 @@ struct Cfg {
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int SMEM = (SHARED ? (RING > MERGE ? RING : MERGE) : RING + MERGE) + QUERY + STATS;
   static_assert(STAGES >= 2, "a chunk in flight while another is used");
-  // shortest run of pages: four chunks a warp (two for one of these runs are no faster, a split costs 3 us)
-  static constexpr int MIN_PAGES = 4 * WARPS * CHUNK / PAGE;
+  // A unit's start and end cost about as much as kUnit pages, and it is cut into pieces of two chunks a warp at least.
+  static constexpr int MIN_PAGES = 2 * WARPS * CHUNK / PAGE > 1 ? 2 * WARPS * CHUNK / PAGE : 1;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
@@ -181,7 +182,14 @@ __device__ __forceinline__ Request request(const AttnFp4Params& p, int b, int ro
   return r;
 }
 __device__ __forceinline__ int64_t weight(const AttnFp4Params& p, const Request& r) {
-  return static_cast<int64_t>(r.tiles) * p.hk * r.pages;
+  return static_cast<int64_t>(r.tiles) * p.hk * (r.pages + kUnit);
+}
+// A unit of `pages` cut `at` its start + at: the page there, moved to an end of the unit where a piece would be short.
+template <int MIN_PAGES>
+__device__ __forceinline__ int cut_page(int64_t at, int pages) {
+  const int64_t page = at - kUnit;
+  if (page < MIN_PAGES) return 0;
+  return page > pages - MIN_PAGES ? pages : static_cast<int>(page);
 }
 
 // a / b of non-negative numbers, short where both are short.
@@ -192,68 +200,74 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 
 // One unit's part in a CTA's run.
 struct Segment {
-  int64_t u0, u1;  // the unit's place among all pages
+  int64_t u0;  // the unit's place among all
   int64_t qs;
-  int b, h, row0, rows, ctx0, kv_end;
-  int pg0, c0, c1;  // first page; chunks with keys that some row sees
-  bool whole;       // all of the unit
+  int b, h, row0, rows, ctx0, kv_end, pages;
+  int c0, c1;        // chunks with keys that some row sees
+  bool whole, head;  // all of the unit; its beginning
 };
-// Walks a CTA's run [pos, end) of the pages laid end to end.  Request b's first page is at `base`; after the first unit
-// each one follows from the last without a division.
+// Walks a CTA's run [pos, end) of the units laid end to end; each one follows from the last without a division.
 struct Cursor {
-  int64_t pos, end, base;
+  int64_t pos, end, next;  // the run, and where the next unit begins
   int b, tile, h;
   Request r;
 };
-template <int ROWS, int CHUNK>
+template <int ROWS, int CHUNK, int MIN_PAGES>
 __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, const Request* table, int table_b, Cursor& c, Segment& s) {
   const int g = p.hq / p.hk;
-  int off = 0;  // pages of the unit that belong to an earlier run
-  if (c.tile < 0) {
-    if (c.pos >= c.end) return false;
-    const int64_t unit = quotient(c.pos - c.base, c.r.pages);
-    off = static_cast<int>(c.pos - c.base - unit * c.r.pages);
-    c.tile = static_cast<int>(quotient(unit, p.hk));
-    c.h = static_cast<int>(unit - static_cast<int64_t>(c.tile) * p.hk);
-    if (p.whole_units && off) {  // it belongs to the run that it begins in
-      c.pos += c.r.pages - off;
-      off = 0;
-      ++c.h;
+  while (true) {
+    if (c.next >= c.end) return false;
+    if (++c.h == p.hk) {
+      c.h = 0;
+      ++c.tile;
     }
-  } else {
-    ++c.h;
+    while (c.tile >= c.r.tiles) {
+      ++c.b;
+      c.r = c.b - table_b < kTable ? table[c.b - table_b] : request(p, c.b, ROWS);
+      c.tile = 0;
+    }
+    s.u0 = c.next;
+    s.pages = c.r.pages;
+    c.next = s.u0 + s.pages + kUnit;
+    // whole units belong to the run that they begin in; others to each run that holds enough of them
+    int pg0, pg1;
+    if (p.whole_units) {
+      if (s.u0 < c.pos) continue;
+      pg0 = 0;
+      pg1 = s.pages;
+    } else {
+      pg0 = s.u0 >= c.pos ? 0 : cut_page<MIN_PAGES>(c.pos - s.u0, s.pages);
+      pg1 = c.next <= c.end ? s.pages : cut_page<MIN_PAGES>(c.end - s.u0, s.pages);
+      if (pg0 >= pg1) continue;
+    }
+    s.head = pg0 == 0;
+    s.whole = s.head && pg1 == s.pages;
+    s.b = c.b;
+    s.h = c.h;
+    s.row0 = c.tile * ROWS;
+    const int64_t left = static_cast<int64_t>(c.r.q_len) * g - s.row0;
+    s.rows = left < ROWS ? static_cast<int>(left) : ROWS;
+    s.qs = c.r.qs;
+    s.ctx0 = c.r.seq - c.r.q_len;
+    int kv = s.ctx0 + (s.row0 + s.rows - 1) / g + 1;  // keys the tile's last row sees
+    kv = kv < 0 ? 0 : (kv < c.r.seq ? kv : c.r.seq);
+    s.kv_end = kv;
+    s.c0 = pg0 * (PAGE / CHUNK);
+    const int last = kv / CHUNK + (kv % CHUNK ? 1 : 0);
+    s.c1 = pg1 * (PAGE / CHUNK) < last ? pg1 * (PAGE / CHUNK) : last;
+    return true;
   }
-  if (c.pos >= c.end) return false;
-  if (c.h == p.hk) {
-    c.h = 0;
-    ++c.tile;
-  }
-  while (c.tile >= c.r.tiles) {
-    ++c.b;
-    c.r = c.b - table_b < kTable ? table[c.b - table_b] : request(p, c.b, ROWS);
-    c.tile = 0;
-  }
-  s.b = c.b;
-  s.h = c.h;
-  s.row0 = c.tile * ROWS;
-  const int64_t left = static_cast<int64_t>(c.r.q_len) * g - s.row0;
-  s.rows = left < ROWS ? static_cast<int>(left) : ROWS;
-  s.u0 = c.pos - off;
-  s.u1 = s.u0 + c.r.pages;
-  s.pg0 = off;
-  const bool to_end = p.whole_units || c.end >= s.u1;
-  const int pg1 = to_end ? c.r.pages : static_cast<int>(c.end - s.u0);
-  s.whole = off == 0 && to_end;
-  c.pos = s.u0 + pg1;
-  s.qs = c.r.qs;
-  s.ctx0 = c.r.seq - c.r.q_len;
-  int kv = s.ctx0 + (s.row0 + s.rows - 1) / g + 1;  // keys the tile's last row sees
-  kv = kv < 0 ? 0 : (kv < c.r.seq ? kv : c.r.seq);
-  s.kv_end = kv;
-  s.c0 = off * (PAGE / CHUNK);
-  const int last = kv / CHUNK + (kv % CHUNK ? 1 : 0);
-  s.c1 = pg1 * (PAGE / CHUNK) < last ? pg1 * (PAGE / CHUNK) : last;
-  return true;
+}
+// The first and the last run that hold a piece of the unit (by the rule of cut_page, on runs of `per`).
+template <int MIN_PAGES>
+__device__ __forceinline__ int2 runs_of(const Segment& s, int64_t per) {
+  const int64_t end = s.u0 + s.pages + kUnit;
+  const int64_t at_end = quotient(end - 1, per);
+  const int64_t a = quotient(s.u0 + kUnit + MIN_PAGES + per - 1, per) - 1;  // its end leaves a piece behind it
+  const int64_t first = a < at_end ? a : at_end;
+  const int64_t z = s.pages >= MIN_PAGES ? quotient(s.u0 + kUnit + s.pages - MIN_PAGES, per) : first;
+  const int64_t last = z < at_end ? z : at_end;
+  return make_int2(static_cast<int>(first), static_cast<int>(last < first ? first : last));
 }
 
 template <int D, int NT>
@@ -347,9 +361,6 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
     __syncthreads();
   }
   __syncthreads();
-  cons.b = start_b;
-  cons.base = start_base;
-  cons.tile = -1;
   {
     const int i = static_cast<int>(threadIdx.x) - start_b;  // start_b + i is this thread's request, if it is among the first
     if (i >= 0 && i < kTable && threadIdx.x < p.B) table[i] = mine;
@@ -357,7 +368,15 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       table[threadIdx.x] = request(p, start_b + threadIdx.x, ROWS);
   }
   __syncthreads();
-  cons.r = table[0];
+  {  // the unit that the run begins in; the cursor stands before it
+    const Request& r = table[0];
+    const int64_t unit = quotient(cons.pos - start_base, r.pages + kUnit);
+    cons.b = start_b;
+    cons.r = r;
+    cons.tile = static_cast<int>(quotient(unit, p.hk));
+    cons.h = static_cast<int>(unit - static_cast<int64_t>(cons.tile) * p.hk) - 1;
+    cons.next = start_base + unit * (r.pages + kUnit);
+  }
 
   // ---------------------------------------------------------------- loads of this warp's chunks
   const uint32_t ring = smem_addr(smem) + warp * STAGES * K::STAGE;
@@ -422,16 +441,26 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   };
   // The row tile's fragments, a warp per 8 rows: lane (g, t) has dimensions [t D/4, (t + 1) D/4) of row g, word u of its
   // codes against query2[half][j][u][lane].
-  auto convert = [&](const Segment& sg, int half) {
-#pragma unroll 1
-    for (int j = warp; j < NT; j += WARPS) {
-      const int n = 8 * j + g;
-      uint4 raw[D / 32];
-      const uint4* src = row_of(sg, n);
+  static_assert(NT <= WARPS, "a warp per 8 rows");
+  struct Rows {
+    uint4 raw[D / 32];
+  };
+  auto load_rows = [&](const Segment& sg) {
+    Rows x;
+    const int n = 8 * warp + g;
+    const bool valid = warp < NT && n < sg.rows;
+    const uint4* src = row_of(sg, valid ? n : 0);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) x.raw[i] = valid ? src[i] : make_uint4(0, 0, 0, 0);
+    return x;
+  };
+  auto convert = [&](const Segment& sg, int half, const Rows& x) {
+    if (warp < NT) {
+      const int j = warp, n = 8 * j + g;
+      const uint4* raw = x.raw;
       uint32_t top = 0;  // largest magnitude's bf16 bits: its exponent is all that is needed
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        raw[i] = n < sg.rows ? src[i] : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
@@ -454,11 +483,12 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       }
     }
   };
-  bool have = next_segment<ROWS, CHUNK>(p, table, start_b, cons, s);
+  bool have = next_segment<ROWS, CHUNK, K::MIN_PAGES>(p, table, start_b, cons, s);
   if (have) {
+    const Rows x = load_rows(s);
     begin(s);  // the first keys are on their way before the queries are looked at
     fetch();
-    convert(s, 0);
+    convert(s, 0, x);
   }
   __syncthreads();
   for (; have; s = sn, ++unit) {
@@ -466,7 +496,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
     const uint4* query = query2 + turn * NT * KW * 32;
     const float* row_scale = row_scale2 + turn * ROWS;
     const int* row_pos = row_pos2 + turn * ROWS;
-    have = next_segment<ROWS, CHUNK>(p, table, start_b, cons, sn);
+    have = next_segment<ROWS, CHUNK, K::MIN_PAGES>(p, table, start_b, cons, sn);
     if (have && warp < NT && 8 * warp + g < sn.rows)
       asm volatile("prefetch.global.L1 [%0];" ::"l"(row_of(sn, 8 * warp + g)));
     // what of the ring could not be filled under the unit before
@@ -704,14 +734,14 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       }
     }
 
-    if (have) convert(sn, turn ^ 1);  // the barriers below stand before its use
+    if (have) convert(sn, turn ^ 1, load_rows(sn));  // the barriers below stand before its use
     // -------------------------------------------------------------- the warps' states become one
     if constexpr (K::SHARED) {  // no copy may land in the merge area
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncthreads();
     }
     const bool whole = s.whole;
-    const int slot = 2 * blockIdx.x + (s.pg0 > 0 ? 0 : 1);
+    const int slot = 2 * blockIdx.x + (s.head ? 1 : 0);
     float* part = p.part_o + static_cast<int64_t>(slot) * ROWS * (D + 2);
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -785,10 +815,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   __syncthreads();
   if (threadIdx.x < opened) {
     const Segment& u = open[threadIdx.x];
-    const int64_t first = quotient(u.u0, per), last = quotient(u.u1 - 1, per);
+    const int2 runs = runs_of<K::MIN_PAGES>(u, per);
     __threadfence();
-    const bool mine = atomicAdd(&p.tickets[first], 1u) == static_cast<unsigned>(last - first);
-    if (mine) p.tickets[first] = 0;
+    const bool mine = atomicAdd(&p.tickets[runs.x], 1u) == static_cast<unsigned>(runs.y - runs.x);
+    if (mine) p.tickets[runs.x] = 0;
     last_flag[threadIdx.x] = mine;
     __threadfence();
   }
@@ -796,7 +826,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   for (int i = 0; i < opened; ++i) {
     if (!last_flag[i]) continue;
     const Segment u = open[i];
-    const int first = static_cast<int>(quotient(u.u0, per)), last = static_cast<int>(quotient(u.u1 - 1, per));
+    const int2 runs = runs_of<K::MIN_PAGES>(u, per);
+    const int first = runs.x, last = runs.y;
     constexpr int DT = D / 32, BATCH = 4;
     auto at = [&](int c) { return p.part_o + static_cast<int64_t>(2 * c + (c == first ? 1 : 0)) * ROWS * (D + 2); };
     for (int row = warp; row < u.rows; row += WARPS) {
