@@ -21,15 +21,18 @@ void fused_add_rms_norm(torch::Tensor x, torch::Tensor residual, torch::Tensor w
 void rope_kv_write(torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin, torch::Tensor k_cache,
                    torch::Tensor v_cache, torch::Tensor slot_mapping, int64_t hq, int64_t hk, int64_t d, int64_t rot);
 // 4-bit KV cache (kv_fp4_bindings.cpp)
-void rope_kv_write_fp4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin,
-                       torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots, int64_t hq, int64_t hk,
-                       int64_t d, int64_t rot, double k_scale, double v_scale);
-void kv_fp4_read(torch::Tensor k_out, torch::Tensor v_out, torch::Tensor k_cache, torch::Tensor v_cache,
-                 torch::Tensor slots, int64_t d, double k_scale, double v_scale);
-void paged_attention_fp4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
-                         torch::Tensor block_tables, torch::Tensor seq_lens, torch::Tensor q_start, int64_t hq,
-                         int64_t d, double scale, int64_t max_q_len, double k_scale, double v_scale, bool invariant);
-void copy_kv_pages(const std::vector<torch::Tensor>& caches, torch::Tensor src, torch::Tensor dst);
+torch::Tensor rope_kv_write_fp4(const torch::Tensor& qkv, const torch::Tensor& positions, const torch::Tensor& cos_sin,
+                                const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& slots,
+                                int64_t hq, int64_t hk, int64_t d, int64_t rot, double k_scale, double v_scale,
+                                const c10::optional<torch::Tensor>& out);
+std::tuple<torch::Tensor, torch::Tensor> kv_fp4_read(const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                                                     const torch::Tensor& slots, int64_t d, double k_scale,
+                                                     double v_scale);
+void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const torch::Tensor& k_cache,
+                         const torch::Tensor& v_cache, const torch::Tensor& block_tables, const torch::Tensor& seq_lens,
+                         const torch::Tensor& q_start, int64_t hq, int64_t d, double scale, int64_t max_q_len,
+                         double k_scale, double v_scale);
+void copy_kv_pages(const py::list& caches, const torch::Tensor& src, const torch::Tensor& dst);
 void silu_mul(torch::Tensor out, torch::Tensor x);
 void embedding(torch::Tensor out, torch::Tensor ids, torch::Tensor table);
 void argmax_rows(torch::Tensor out, torch::Tensor logits);

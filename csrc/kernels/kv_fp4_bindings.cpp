@@ -1,9 +1,11 @@
 // Python bindings of the 4-bit KV cache: writer, reader, paged attention, page copies.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -81,14 +83,16 @@ Scratch scratch(const torch::Tensor& like, cudaStream_t stream, int64_t floats, 
 
 }  // namespace
 
-void rope_kv_write_fp4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin,
-                       torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots, int64_t hq, int64_t hk,
-                       int64_t d, int64_t rot, double k_scale, double v_scale) {
+torch::Tensor rope_kv_write_fp4(const torch::Tensor& qkv, const torch::Tensor& positions, const torch::Tensor& cos_sin,
+                                const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& slots,
+                                int64_t hq, int64_t hk, int64_t d, int64_t rot, double k_scale, double v_scale,
+                                const c10::optional<torch::Tensor>& out) {
   const char* who = "rope_kv_write_fp4";
   check_dim(d, who);
   check_cache(k_cache, v_cache, d, who);
   TORCH_CHECK(hq > 0 && hk > 0 && k_cache.size(1) == hk, who, ": the caches hold ", k_cache.size(1), " kv heads, not ", hk);
   check_rows(qkv, (hq + 2 * hk) * d, k_cache, who, "qkv");
+  const torch::Tensor q_out = out.has_value() ? *out : torch::empty({qkv.size(0), hq * d}, qkv.options());
   check_rows(q_out, hq * d, k_cache, who, "q_out");
   TORCH_CHECK(q_out.size(0) == qkv.size(0), who, ": one q_out row per token");
   TORCH_CHECK(!q_out.is_alias_of(qkv), who, ": q_out must not share qkv's memory (a rotation reads both halves)");
@@ -100,7 +104,7 @@ void rope_kv_write_fp4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor pos
                   cos_sin.is_contiguous() && cos_sin.device() == k_cache.device() && cos_sin.size(0) > 0,
               who, ": cos_sin must be f32 [positions, rot] contiguous");
   TORCH_CHECK(k_scale > 0 && v_scale > 0, who, ": cache scales must be positive");
-  if (qkv.size(0) == 0) return;
+  if (qkv.size(0) == 0) return q_out;
   const c10::cuda::CUDAGuard guard(k_cache.device());
   KvFp4WriteParams p{};
   p.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv.data_ptr());
@@ -122,21 +126,21 @@ void rope_kv_write_fp4(torch::Tensor q_out, torch::Tensor qkv, torch::Tensor pos
   p.v_inv = static_cast<float>(1.0 / v_scale);
   const int r = sh_kv_fp4_write(&p, static_cast<int>(d), at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(r == 0, "sh_kv_fp4_write failed with code ", r);
+  return q_out;
 }
 
-void kv_fp4_read(torch::Tensor k_out, torch::Tensor v_out, torch::Tensor k_cache, torch::Tensor v_cache,
-                 torch::Tensor slots, int64_t d, double k_scale, double v_scale) {
+std::tuple<torch::Tensor, torch::Tensor> kv_fp4_read(const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                                                     const torch::Tensor& slots, int64_t d, double k_scale,
+                                                     double v_scale) {
   const char* who = "kv_fp4_read";
   check_dim(d, who);
   check_cache(k_cache, v_cache, d, who);
   check_index(slots, at::kLong, 1, k_cache, who, "slots");
-  for (const torch::Tensor* o : {&k_out, &v_out})
-    TORCH_CHECK(o->scalar_type() == at::kBFloat16 && o->is_contiguous() && o->device() == k_cache.device() &&
-                    o->dim() == 3 && o->size(0) == slots.numel() && o->size(1) == k_cache.size(1) && o->size(2) == d &&
-                    reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0,
-                who, ": outputs bf16 [slots, kv_heads, head_dim] contiguous");
-  if (slots.numel() == 0) return;
   const c10::cuda::CUDAGuard guard(k_cache.device());
+  const auto options = k_cache.options().dtype(at::kBFloat16);
+  const torch::Tensor k_out = torch::empty({slots.numel(), k_cache.size(1), d}, options);
+  const torch::Tensor v_out = torch::empty({slots.numel(), k_cache.size(1), d}, options);
+  if (slots.numel() == 0) return {k_out, v_out};
   KvFp4ReadParams p{};
   p.k_cache = k_cache.data_ptr<uint8_t>();
   p.v_cache = v_cache.data_ptr<uint8_t>();
@@ -150,12 +154,16 @@ void kv_fp4_read(torch::Tensor k_out, torch::Tensor v_out, torch::Tensor k_cache
   p.v_scale = static_cast<float>(v_scale);
   const int r = sh_kv_fp4_read(&p, static_cast<int>(d), at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(r == 0, "sh_kv_fp4_read failed with code ", r);
+  return {k_out, v_out};
 }
 
-void paged_attention_fp4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
-                         torch::Tensor block_tables, torch::Tensor seq_lens, torch::Tensor q_start, int64_t hq,
-                         int64_t d, double scale, int64_t max_q_len, double k_scale, double v_scale, bool invariant) {
+void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const torch::Tensor& k_cache,
+                         const torch::Tensor& v_cache, const torch::Tensor& block_tables, const torch::Tensor& seq_lens,
+                         const torch::Tensor& q_start, int64_t hq, int64_t d, double scale, int64_t max_q_len,
+                         double k_scale, double v_scale) {
   const char* who = "paged_attention_fp4";
+  const char* env = std::getenv("SH_BATCH_INVARIANT");
+  const bool invariant = env != nullptr && env[0] == '1' && env[1] == 0;
   check_dim(d, who);
   check_cache(k_cache, v_cache, d, who);
   const int64_t hk = k_cache.size(1), B = seq_lens.numel();
@@ -221,35 +229,44 @@ void paged_attention_fp4(torch::Tensor out, torch::Tensor q, torch::Tensor k_cac
   TORCH_CHECK(r == 0, "sh_paged_attention_fp4 failed with code ", r);
 }
 
-void copy_kv_pages(const std::vector<torch::Tensor>& caches, torch::Tensor src, torch::Tensor dst) {
+// The list is walked in place: an engine passes two tensors a layer, and a copy of each would cost as much as the call.
+void copy_kv_pages(const py::list& caches, const torch::Tensor& src, const torch::Tensor& dst) {
   const char* who = "copy_kv_pages";
-  TORCH_CHECK(!caches.empty() && caches[0].is_cuda(), who, ": at least one CUDA cache tensor");
-  check_index(src, at::kLong, 1, caches[0], who, "src");
-  check_index(dst, at::kLong, 1, caches[0], who, "dst");
+  const Py_ssize_t count = PyList_GET_SIZE(caches.ptr());
+  auto cache = [&](Py_ssize_t i) -> const at::Tensor& {
+    PyObject* o = PyList_GET_ITEM(caches.ptr(), i);
+    TORCH_CHECK_TYPE(THPVariable_Check(o), who, ": caches must be tensors");
+    return THPVariable_Unpack(o);
+  };
+  TORCH_CHECK(count > 0 && cache(0).is_cuda(), who, ": at least one CUDA cache tensor");
+  const c10::Device device = cache(0).device();
+  check_index(src, at::kLong, 1, cache(0), who, "src");
+  check_index(dst, at::kLong, 1, cache(0), who, "dst");
   TORCH_CHECK(src.numel() == dst.numel(), who, ": ", src.numel(), " sources for ", dst.numel(), " destinations");
-  for (const torch::Tensor& c : caches) {
-    TORCH_CHECK(c.device() == caches[0].device() && c.dim() >= 2 && c.is_contiguous(), who,
+  std::vector<KvCopyParams> calls((count + SH_KV_COPY_MAX_TENSORS - 1) / SH_KV_COPY_MAX_TENSORS);
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    const at::Tensor& c = cache(i);
+    TORCH_CHECK(c.device() == device && c.dim() >= 2 && c.is_contiguous(), who,
                 ": cache tensors [num_blocks, ...] contiguous on one device");
-    TORCH_CHECK(c.numel() == 0 || ((c.numel() / c.size(0)) * c.element_size() % 16 == 0 &&
-                                   reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0),
-                who, ": pages must be multiples of 16 bytes and 16-byte aligned");
+    const int64_t n = c.numel();
+    if (n == 0) continue;
+    const int64_t bytes = n / c.size(0) * static_cast<int64_t>(c.element_size());
+    uint8_t* base = static_cast<uint8_t*>(c.data_ptr());
+    TORCH_CHECK(bytes % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0, who,
+                ": pages must be multiples of 16 bytes and 16-byte aligned");
+    KvCopyParams& p = calls[i / SH_KV_COPY_MAX_TENSORS];
+    p.base[p.tensors] = base;
+    p.page_bytes[p.tensors] = bytes;
+    p.pages[p.tensors] = c.size(0);
+    ++p.tensors;
   }
   if (src.numel() == 0) return;
-  const c10::cuda::CUDAGuard guard(caches[0].device());
+  const c10::cuda::CUDAGuard guard(device);
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  for (size_t at = 0; at < caches.size(); at += SH_KV_COPY_MAX_TENSORS) {
-    KvCopyParams p{};
+  for (KvCopyParams& p : calls) {
     p.src = src.data_ptr<int64_t>();
     p.dst = dst.data_ptr<int64_t>();
     p.n = src.numel();
-    for (size_t i = at; i < caches.size() && i < at + SH_KV_COPY_MAX_TENSORS; ++i) {
-      const torch::Tensor& c = caches[i];
-      if (c.numel() == 0) continue;
-      p.base[p.tensors] = static_cast<uint8_t*>(c.data_ptr());
-      p.page_bytes[p.tensors] = (c.numel() / c.size(0)) * c.element_size();
-      p.pages[p.tensors] = c.size(0);
-      ++p.tensors;
-    }
     const int r = sh_kv_copy_pages(&p, stream);
     TORCH_CHECK(r == 0, "sh_kv_copy_pages failed with code ", r);
   }

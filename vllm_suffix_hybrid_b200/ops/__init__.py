@@ -196,11 +196,8 @@ def rope_kv_write_fp4(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, h
         q = ref.rope_kv_write_fp4(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, hq, hk, d, rot, k_scale,
                                   v_scale)
         return q if q_out is None else q_out.copy_(q)
-    if q_out is None:
-        q_out = torch.empty(qkv.shape[0], hq * d, dtype=qkv.dtype, device=qkv.device)
-    native().rope_kv_write_fp4(q_out, qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, hq, hk, d, rot, k_scale,
-                               v_scale)
-    return q_out
+    return native().rope_kv_write_fp4(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, hq, hk, d, rot, k_scale,
+                                      v_scale, q_out)
 
 
 def kv_fp4_read(k_cache, v_cache, slots, d, k_scale: float = 1.0, v_scale: float = 1.0):
@@ -208,10 +205,7 @@ def kv_fp4_read(k_cache, v_cache, slots, d, k_scale: float = 1.0, v_scale: float
     outside the cache."""
     if not _cuda(k_cache):
         return ref.kv_fp4_read(k_cache, slots, d, k_scale), ref.kv_fp4_read(v_cache, slots, d, v_scale)
-    k = torch.empty(slots.shape[0], k_cache.shape[1], d, dtype=torch.bfloat16, device=k_cache.device)
-    v = torch.empty_like(k)
-    native().kv_fp4_read(k, v, k_cache, v_cache, slots, d, k_scale, v_scale)
-    return k, v
+    return native().kv_fp4_read(k_cache, v_cache, slots, d, k_scale, v_scale)
 
 
 def paged_attention_fp4(out, q, k_cache, v_cache, block_tables, seq_lens, q_start, hq, d, scale, max_q_len: int,
@@ -228,7 +222,7 @@ def paged_attention_fp4(out, q, k_cache, v_cache, block_tables, seq_lens, q_star
                                                          seq_lens, q_start, hq, d, scale, k_scale, v_scale))
         return out
     native().paged_attention_fp4(out, q, k_cache, v_cache, block_tables, seq_lens, q_start, hq, d, scale, max_q_len,
-                                 k_scale, v_scale, os.environ.get("SH_BATCH_INVARIANT", "0") == "1")
+                                 k_scale, v_scale)
     return out
 
 
@@ -237,7 +231,7 @@ def copy_kv_pages(caches, src: torch.Tensor, dst: torch.Tensor) -> None:
 
     src, dst: int64 [n] block ids on the caches' device; a pair with an id outside a tensor is skipped.  No id may
     be a destination twice, or both a source and a destination (the copies run in no order)."""
-    caches = list(caches)
+    caches = caches if type(caches) is list else list(caches)
     if not caches:
         return
     if not _cuda(caches[0]):
