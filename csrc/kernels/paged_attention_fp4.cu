@@ -54,15 +54,16 @@ struct Geo {
 };
 // Warps of a CTA, CTAs of an SM, 16-token groups of a warp step (a chunk) and ring stages.  O^T takes D / 4 registers a
 // thread for every 8 rows: with 32 of them a thread fits 128 registers and an SM 16 warps, beyond that 8 (255).  At
-// head_dim 128 those 16 are four CTAs, whose starts, merges and ends fall under one another's streaming (decode
-// 64 x 2048: 42 us against 48 with two CTAs of 8); at 64 two are better (64 x 4096: 20 us against 23).
+// head_dim 128 the CTAs have 4 warps, so that their starts, merges and ends fall under one another's streaming (decode
+// 64 x 2048: 42 us against 48 with CTAs of 8; 32 rows over 32 x 6000: 142 against 153); elsewhere 8 are better (decode
+// 64 x 4096 at 64: 20 us against 23, 24 x 4000 at 256: 24 against 33).  Twelve or sixteen warps for the wider tiles, or
+// a pair of warps to share a tile's dimensions, were slower (24 rows: 157 and 131 us against 109): they spill.
 template <int D, int NT>
 struct Cfg {
   static constexpr int REGS_O = D / 4 * NT;
   static constexpr int SUB = REGS_O <= 96 && NT <= 3 ? 2 : 1;
-  static constexpr bool QUADS = D == 128 && NT == 1;
-  static constexpr int CTAS = QUADS ? 4 : (REGS_O <= 32 ? 2 : 1);
-  static constexpr int WARPS = QUADS ? 4 : 8;
+  static constexpr int WARPS = D == 128 ? 4 : 8;
+  static constexpr int CTAS = (REGS_O <= 32 ? 16 : 8) / WARPS;
   static constexpr int THREADS = WARPS * 32;
   static constexpr int CHUNK = 16 * SUB;
   static constexpr int CODES = CHUNK * Geo<D>::ROW;
