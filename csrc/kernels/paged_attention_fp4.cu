@@ -291,6 +291,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   __shared__ int64_t start_base;
   __shared__ int start_b;
   __shared__ Request table[kTable];  // of requests start_b, start_b + 1, ...
+  __shared__ Cursor cursor;
+  __shared__ Segment segs[3];  // this unit, the next one and the one behind it, found by thread 0
+  __shared__ int seg_ok[3];
   __shared__ Segment open[2];  // units that this CTA has a partial of: at most the run's first and last
   __shared__ int last_flag[2];
 
@@ -340,20 +343,17 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   total += done;
   int64_t per = quotient(total + gridDim.x - 1, gridDim.x);
   if (per < K::MIN_PAGES) per = K::MIN_PAGES;
-  Cursor cons;
-  cons.pos = per * blockIdx.x;
-  cons.end = cons.pos + per;
-  if (cons.end > total) cons.end = total;
-  if (cons.pos >= cons.end) return;
-  if (incl - first_w <= cons.pos && cons.pos < incl) {
+  const int64_t run = per * blockIdx.x;
+  if (run >= total) return;
+  if (incl - first_w <= run && run < incl) {
     start_b = threadIdx.x;
     start_base = incl - first_w;
   }
-  for (int64_t b0 = THREADS; done <= cons.pos; b0 += THREADS) {
+  for (int64_t b0 = THREADS; done <= run; b0 += THREADS) {
     const int64_t b = b0 + threadIdx.x;
     const int64_t w = b < p.B ? weight(p, request(p, static_cast<int>(b), ROWS)) : 0;
     incl = done + scan_warps(w);
-    if (incl - w <= cons.pos && cons.pos < incl) {
+    if (incl - w <= run && run < incl) {
       start_b = static_cast<int>(b);
       start_base = incl - w;
     }
@@ -369,15 +369,28 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       table[threadIdx.x] = request(p, start_b + threadIdx.x, ROWS);
   }
   __syncthreads();
-  {  // the unit that the run begins in; the cursor stands before it
-    const Request& r = table[0];
-    const int64_t unit = quotient(cons.pos - start_base, r.pages + kUnit);
-    cons.b = start_b;
-    cons.r = r;
-    cons.tile = static_cast<int>(quotient(unit, p.hk));
-    cons.h = static_cast<int>(unit - static_cast<int64_t>(cons.tile) * p.hk) - 1;
-    cons.next = start_base + unit * (r.pages + kUnit);
+  auto advance = [&](int slot) {  // thread 0: the next unit of the run
+    Cursor c = cursor;
+    Segment sg;
+    seg_ok[slot] = next_segment<ROWS, CHUNK, K::MIN_PAGES>(p, table, start_b, c, sg);
+    segs[slot] = sg;
+    cursor = c;
+  };
+  if (threadIdx.x == 0) {  // the unit that the run begins in; the cursor stands before it
+    Cursor c;
+    c.pos = run;
+    c.end = run + per < total ? run + per : total;
+    c.r = table[0];
+    const int64_t unit = quotient(run - start_base, c.r.pages + kUnit);
+    c.b = start_b;
+    c.tile = static_cast<int>(quotient(unit, p.hk));
+    c.h = static_cast<int>(unit - static_cast<int64_t>(c.tile) * p.hk) - 1;
+    c.next = start_base + unit * (c.r.pages + kUnit);
+    cursor = c;
+    advance(0);
+    advance(1);
   }
+  __syncthreads();
 
   // ---------------------------------------------------------------- loads of this warp's chunks
   const uint32_t ring = smem_addr(smem) + warp * STAGES * K::STAGE;
@@ -433,7 +446,6 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   const int vsoff = 2 * K::CODES + K::SCALES + 2 * t * G::SROW + (D == 64 ? g >> 1 : (D == 128 ? g : 2 * g));
 
   // ---------------------------------------------------------------- segments
-  Segment s, sn;
   int opened = 0, unit = 0;  // partials left and units done so far; unit's parity: its half of query2
   auto row_of = [&](const Segment& sg, int n) {  // row n's queries, this lane's dimensions
     const int rr = sg.row0 + n;
@@ -484,20 +496,21 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       }
     }
   };
-  bool have = next_segment<ROWS, CHUNK, K::MIN_PAGES>(p, table, start_b, cons, s);
-  if (have) {
-    const Rows x = load_rows(s);
-    begin(s);  // the first keys are on their way before the queries are looked at
+  if (seg_ok[0]) {
+    const Rows x = load_rows(segs[0]);
+    begin(segs[0]);  // the first keys are on their way before the queries are looked at
     fetch();
-    convert(s, 0, x);
+    convert(segs[0], 0, x);
   }
   __syncthreads();
-  for (; have; s = sn, ++unit) {
-    const int turn = unit & 1;
+  for (; seg_ok[unit % 3]; ++unit) {
+    const Segment& s = segs[unit % 3];
+    const Segment& sn = segs[(unit + 1) % 3];
+    const bool have = seg_ok[(unit + 1) % 3];
+    const int turn = unit & 1, c_end = s.c1, kv_end = s.kv_end;
     const uint4* query = query2 + turn * NT * KW * 32;
     const float* row_scale = row_scale2 + turn * ROWS;
     const int* row_pos = row_pos2 + turn * ROWS;
-    have = next_segment<ROWS, CHUNK, K::MIN_PAGES>(p, table, start_b, cons, sn);
     if (have && warp < NT && 8 * warp + g < sn.rows)
       asm volatile("prefetch.global.L1 [%0];" ::"l"(row_of(sn, 8 * warp + g)));
     // what of the ring could not be filled under the unit before
@@ -520,7 +533,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       for (int i = 0; i < MT; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
 
 #pragma unroll 1
-    for (int c = s.c0 + warp; c < s.c1; c += WARPS, ++it) {
+    for (int c = s.c0 + warp; c < c_end; c += WARPS, ++it) {
       // a group per chunk: with a full ring STAGES - 2 later ones may still be under way
       if (asked - it < STAGES - 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
       else asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
@@ -705,8 +718,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
             b = sp[G::SROW];
           }
           if (edge) {  // a token that no sequence owns: its codes are finite, its scale may be anything
-            if (key0 + r + 2 * t >= s.kv_end) a = 0;
-            if (key0 + r + 2 * t + 1 >= s.kv_end) b = 0;
+            if (key0 + r + 2 * t >= kv_end) a = 0;
+            if (key0 + r + 2 * t + 1 >= kv_end) b = 0;
           }
           if constexpr (D == 256) {
             vsc[pr][0] = e4m3x2(__byte_perm(a, b, 0x0040));
@@ -735,7 +748,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       }
     }
 
-    if (have) convert(sn, turn ^ 1, load_rows(sn));  // the barriers below stand before its use
+    // (the barriers below stand before the use of both)
+    if (have) convert(sn, turn ^ 1, load_rows(sn));
+    if (threadIdx.x == 0 && have) advance((unit + 2) % 3);
+    else if (threadIdx.x == 0) seg_ok[(unit + 2) % 3] = 0;
     // -------------------------------------------------------------- the warps' states become one
     if constexpr (K::SHARED) {  // no copy may land in the merge area
       asm volatile("cp.async.wait_all;" ::: "memory");
