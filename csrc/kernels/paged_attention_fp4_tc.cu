@@ -45,6 +45,7 @@ constexpr int MMA_WARP = 8 + 2 * PRODUCERS;
 constexpr int THREADS = (MMA_WARP + 2) * 32;
 constexpr float kSlack = 8.f;
 constexpr int kMergeDims = 16;
+constexpr int kMinTiles = 4;  // shortest piece of a unit that is cut
 constexpr int kUnit = 512;  // a unit's start and end in keys (measured: 256 and 1024 leave the SMs less even)
 
 template <int D>
@@ -234,11 +235,20 @@ __device__ __forceinline__ int64_t cost(const Request& r, int group, int64_t n) 
   return n * (r.ctx + kUnit) * group + ROWS * (n * (n + 1) / 2);
 }
 
+// A unit of `tiles` key tiles and cost w, cut where `at` of w lies behind: the tile there, moved to an end of the unit
+// where a piece would be short.
+__device__ __forceinline__ int cut_tile(int64_t at, int64_t tiles, int64_t w) {
+  const int64_t t = at * tiles / w;
+  if (t < kMinTiles) return 0;
+  return static_cast<int>(t > tiles - kMinTiles ? tiles : t);
+}
+
 struct Segment {
   int64_t u0, u1;  // the unit's place among all costs
   int64_t qs, ctx0, kv_end;
   int b, h, row0, rows, k0, k1;  // key tiles [k0, k1) of the unit
   bool whole, head;              // all of the unit; its beginning
+  bool none;                     // this run has no part in it
 };
 // Walks a CTA's run [pos, end) of the units laid end to end.  Request b begins at `base`; after the first unit, which
 // is searched for, each one follows from the last without a division.
@@ -286,10 +296,12 @@ __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, 
   const int64_t tiles = (kv + KT - 1) / KT, w = tile_cost<ROWS>(c.r, g, c.tile);
   s.u0 = c.pos - r0;
   s.u1 = s.u0 + w;
-  s.head = r0 == 0;
-  s.whole = s.head && c.end >= s.u1;
-  s.k0 = s.head ? 0 : static_cast<int>(r0 * tiles / w);
-  s.k1 = c.end >= s.u1 ? static_cast<int>(tiles) : static_cast<int>((c.end - s.u0) * tiles / w);
+  s.k0 = r0 == 0 ? 0 : cut_tile(r0, tiles, w);
+  s.k1 = c.end >= s.u1 ? static_cast<int>(tiles) : cut_tile(c.end - s.u0, tiles, w);
+  // a piece without tiles is nobody's, but a unit without any belongs to the run that ends it
+  s.none = s.k0 >= s.k1 && !(tiles == 0 && c.end >= s.u1);
+  s.head = s.k0 == 0;
+  s.whole = s.head && s.k1 == tiles;
   c.pos = c.end < s.u1 ? c.end : s.u1;
   return true;
 }
@@ -316,7 +328,9 @@ __device__ __forceinline__ int64_t find_run(const AttnFp4Params& p, int run, int
   total = 0;
   for (int w = 0; w < N / 32; ++w) total += scan[w];
   __syncthreads();
-  const int64_t per = (total + runs - 1) / runs;
+  int64_t per = (total + runs - 1) / runs;
+  const int64_t least = static_cast<int64_t>(kMinTiles) * KT * group;  // a run in the middle of a unit is never without a tile
+  if (per < least) per = least;
   cur.pos = per * run;
   cur.end = cur.pos + per < total ? cur.pos + per : total;
   cur.tile = -1;
@@ -362,6 +376,13 @@ __device__ __forceinline__ Split* splits(const AttnFp4Params& p, int runs) {
 template <int D>
 __device__ __forceinline__ float* partial(const AttnFp4Params& p, int c, bool begins, int q, int row) {
   return p.part_o + (static_cast<int64_t>(2 * c + (begins ? 1 : 0)) * Smem<D>::NQ + q) * (D + 2) * 128 + row;
+}
+
+// The last run that holds a piece of a unit that is cut: cut_tile of its beginning leaves tiles behind.
+__device__ __forceinline__ int last_run(const Segment& s, int64_t per) {
+  const int64_t w = s.u1 - s.u0, tiles = (s.kv_end + KT - 1) / KT;
+  const int64_t at = (w * (tiles - kMinTiles + 1) - 1) / tiles;  // the last place with floor(at tiles / w) <= tiles - kMinTiles
+  return static_cast<int>((s.u0 + at) / per);
 }
 
 // Eight values, one 16-byte chunk: 8 codes times their block's scale.
@@ -450,7 +471,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
     auto settle = [&]() {  // the next unit with keys
       do {
         more = next_segment<ROWS>(p, cur, s);
-      } while (more && s.k0 == s.k1);
+      } while (more && s.k0 >= s.k1);
       kt = s.k0;
       if (more) {
         blk = block_of(kt);
@@ -544,7 +565,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
       const bool more = next_segment<ROWS>(p, cur, s);
       if (!__shfl_sync(0xffffffffu, static_cast<int>(more), 0)) break;
       const bool mine = __shfl_sync(0xffffffffu, s.rows, 0) > q * 128;  // this tile has rows
-      const int tiles = __shfl_sync(0xffffffffu, s.k1 - s.k0, 0);
+      const int tiles = __shfl_sync(0xffffffffu, max(s.k1 - s.k0, 0), 0);
       if (tiles > 0 && mine) {
         ok = wait(&qfull[q], qc & 1);
         ++qc;
@@ -620,7 +641,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
       bool more;
       do {
         more = next_segment<ROWS>(p, cur, sg);
-      } while (more && q * 128 >= sg.rows);
+      } while (more && (q * 128 >= sg.rows || sg.none));
       return more;
     };
     auto scan_row = [&](const Segment& sg) {
@@ -798,7 +819,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
         continue;
       }
       if (q == 0 && r == 0 && s.head)
-        splits<D>(p, gridDim.x)[blockIdx.x] = {s.qs, static_cast<int>((s.u1 - 1) / per), s.rows, s.row0, s.h};
+        splits<D>(p, gridDim.x)[blockIdx.x] = {s.qs, last_run(s, per), s.rows, s.row0, s.h};
       float* mine = partial<D>(p, blockIdx.x, s.head, q, r);
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {

@@ -130,6 +130,15 @@ def test_many_rows(hq, hk, d, q, seqs):
     check(c, attend(c))
 
 
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (4, 4, 64), (16, 2, 256), (7, 1, 128), (40, 1, 64)])
+@pytest.mark.parametrize("q,seqs", [((90,), (100,)), ((90,), (256,)), ((70,), (320,)), ((70, 66, 1, 0), (30, 513, 255, 70)),
+                                    ((130,), (2048,)), ((3, 40, 0, 129), (300, 0, 900, 129))])
+def test_many_rows_in_a_wide_table(hq, hk, d, q, seqs):
+    """A table far wider than its lengths says that the work may be large: few short units for many CTAs."""
+    c = case(q, seqs, hq, hk, d, seed=30 + d, cols=4000)
+    check(c, attend(c))
+
+
 def test_many_rows_that_see_nothing():
     c = case((90, 70, 40), (30, 0, 40), 8, 2, 128, seed=21)
     got = attend(c)
