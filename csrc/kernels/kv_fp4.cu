@@ -4,7 +4,9 @@
 //   s = e4m3(clamp(max|x'| / 6, 2^-9, 448)),  code = e2m1(x' / s)   (both to nearest even, saturating)
 // The floor keeps the scale of a block of zeros a positive number; with it, or with values beyond 2688 (infinities
 // among them), codes saturate and the cache stays finite.  A NaN is stored as the block's largest magnitude.
+#include <float.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -18,8 +20,12 @@ namespace kv4 {
 
 constexpr int PAGE = 64;
 constexpr int WRITE_THREADS = 256;
-// Below, 256 threads a token, else 32 (head_dim 128: 768 tokens take 8.2 us against 10.4, 1500 take 15.7 against 12.2).
-constexpr int64_t kFewTokens = 1200;
+// Below, 256 threads a token, from there the kernel whose warps each take a run of heads.  In us for 420, 600, 900 and 1200
+// tokens: 32 + 2 x 8 heads of 128: 3.7, 5.4, 6.8, 8.9 against 6.2, 6.8, 7.7, 8.8; as many of 256: 6.8, 10.9, 16.2, 19.4 against
+// 8.3, 9.9, 12.6, 14.4; 8 + 2 x 2 of 64: 3.1, 5.1, 6.3, 7.4 against 3.2, 3.6, 3.9, 4.6.
+constexpr int64_t kFewTokens = 600;
+constexpr int STREAM_CTAS = 2, DEPTH = 4;
+constexpr int READ_THREADS = 128, READ_UNITS = 4;
 
 template <int D>
 struct Geo {
@@ -54,6 +60,33 @@ __device__ __forceinline__ void put_query(__nv_bfloat16* dst, const float* x) {
   d[0] = make_uint4(w[0], w[1], w[2], w[3]);
   d[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
+// The block's scale, and codes of x / scale.  The quotient is x (rh + rl) with rh + rl = 1 / scale in two words, rounded
+// once (but for 2^-24 of a unit).  The ties t between codes have at most 3 bits and a scale 4, so t * scale is exact; if x
+// is that, the result is t; the next x is further away than the rounding reaches: every code is that of the true
+// quotient.  One product with rh alone moves values off their ties; a division per value made the writer's arithmetic a
+// third longer (16384 tokens of 48 heads of 128: 32 million warp instructions).
+struct Scale {
+  __nv_fp8_e4m3 e4m3;
+  float s, rh, rl;
+};
+__device__ __forceinline__ Scale block_scale(float amax) {
+  Scale r;
+  r.e4m3 = __nv_fp8_e4m3(fminf(fmaxf(__fdiv_rn(amax, 6.f), 1.f / 512.f), 448.f));
+  r.s = static_cast<float>(r.e4m3);
+  r.rh = __frcp_rn(r.s);
+  r.rl = __fmul_rn(__fmaf_rn(-r.rh, r.s, 1.f), r.rh);
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void quotients(float* x, float amax, const Scale& sc) {
+  if (amax <= FLT_MAX) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(x[i], sc.rh, __fmul_rn(x[i], sc.rl));
+  } else {  // an infinity times a zero rl would be no number
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __fmul_rn(x[i], sc.rh);
+  }
+}
 // A block of 16 key or value dimensions into its page (block blk of token off).
 template <int D>
 __device__ __forceinline__ void put_cached(uint8_t* page, int off, int blk, float* x, float inv) {
@@ -63,23 +96,18 @@ __device__ __forceinline__ void put_cached(uint8_t* page, int off, int blk, floa
     x[i] = __fmul_rn(x[i], inv);
     amax = fmaxf(amax, fabsf(x[i]));
   }
-  const __nv_fp8_e4m3 sc(fminf(fmaxf(__fdiv_rn(amax, 6.f), 1.f / 512.f), 448.f));
-  const float sf = static_cast<float>(sc);
-  // a true quotient: multiplying by 1/s moves values that lie between two codes off their tie
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = __fdiv_rn(x[i], sf);
+  const Scale sc = block_scale(amax);
+  quotients<16>(x, amax, sc);
   *reinterpret_cast<uint2*>(page + off * Geo<D>::ROW + blk * 8) = make_uint2(nvq::e2m1x8(x), nvq::e2m1x8(x + 8));
-  page[PAGE * Geo<D>::ROW + off * Geo<D>::SROW + blk] = sc.__x;
+  page[PAGE * Geo<D>::ROW + off * Geo<D>::SROW + blk] = sc.e4m3.__x;
 }
 
 // TPT threads a token.  The rotation pairs dimension d < rot/2 with d + rot/2: where rot/2 is a whole number of blocks
 // (WHOLE) a thread takes a block and its partner, reads their cosines and sines once and keeps them through its heads
 // (every TPT / items-th one); the blocks behind rot go as they are.  Otherwise each block fetches its partners singly.
 //
-// Memory bound: 16384 tokens of 32 + 2 x 8 heads of 128 (363 MB) take 86 us, 65% of the copy rate; what is left is the
-// loads in flight, which 121 registers a thread hold to 16 warps an SM (at 80 registers it spills: 96 us; fetching a
-// head ahead takes 139: 165 us).  With 32 threads a token a thread's cosines serve five heads; with 256 a single token's
-// heads are all in flight.
+// Bound by latency: a single token of 32 + 2 x 8 heads of 128 takes 2.4 us, 389 take 3.7.  With 256 threads a token all
+// of its heads are in flight.
 template <int D, int TPT, bool WHOLE>
 __global__ void __launch_bounds__(WRITE_THREADS, (TPT == 32 && D < 256 ? 2 : 3)) write_kernel(KvFp4WriteParams p) {
   constexpr int BLOCKS = D / 16;
@@ -163,45 +191,219 @@ __global__ void __launch_bounds__(WRITE_THREADS, (TPT == 32 && D < 256 ? 2 : 3))
   }
 }
 
-// One thread per (slot, head, 16-dimension block).
+// Eight dimensions, a thread's unit in the kernels below: one 16-byte access.
+__device__ __forceinline__ void unpack8(const uint4& r, float* v) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint4 pack8(const float* x) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// A unit of a key or value into its page, with the other half of its block, which lane ^ 1 brings; the whole warp calls.
 template <int D>
-__global__ void __launch_bounds__(256) read_kernel(KvFp4ReadParams p) {
-  constexpr int BLOCKS = D / 16;
+__device__ __forceinline__ void put_unit(uint8_t* page, int off, int unit, float* x, float inv, bool live) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = __fmul_rn(x[i], inv);
+    amax = fmaxf(amax, fabsf(x[i]));
+  }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  const Scale sc = block_scale(amax);
+  quotients<8>(x, amax, sc);
+  if (!live) return;
+  *reinterpret_cast<uint32_t*>(page + off * Geo<D>::ROW + unit * 4) = nvq::e2m1x8(x);
+  if (!(unit & 1)) page[PAGE * Geo<D>::ROW + off * Geo<D>::SROW + (unit >> 1)] = sc.e4m3.__x;
+}
+
+__device__ __forceinline__ void async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Many tokens.  A token is a row of steps of STEP heads each, queries, keys and values.  A lane holds two units of a head:
+// one and the unit that it is rotated with, or two behind rot (or of a value), so that the blocks' halves are neighbours.
+// The steps of all tokens, end to end, are cut into one run per warp.  A lane copies what it will read into its own
+// places of shared memory, DEPTH - 1 steps ahead: loads are always in flight and nobody waits for another thread.
+//
+// Memory bound.  16384 tokens of 32 + 2 x 8 heads of 128 (363 MB with the cosines) take 72 us, 78% of the copy rate, of
+// 16 + 2 x 2 heads of 256 (303 MB) 57 us, 82%; 256 threads a token take 117 and 137 there, and a warp a token with its
+// loads in registers 87 and 125.  (Three CTAs an SM, three or two steps deep: the same for many tokens, 1 us more for a
+// thousand; four CTAs, two deep: 97, for 64 registers spill.)
+template <int D>
+__global__ void __launch_bounds__(WRITE_THREADS, STREAM_CTAS) write_stream_kernel(KvFp4WriteParams p) {
+  constexpr int UNITS = D / 8, ITEMS = UNITS / 2, STEP = 32 / ITEMS;
+  extern __shared__ uint4 ring[];  // [DEPTH][6][WRITE_THREADS]: the two units, cosines (2), sines (2)
   shk::pdl_trigger();
   shk::pdl_wait();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t rows = p.n * p.hk;
-  if (i >= rows * BLOCKS) return;
-  const bool key = blockIdx.y == 0;
-  const int blk = static_cast<int>(i % BLOCKS);
-  const int64_t row = i / BLOCKS;
-  const int64_t slot = p.slots[row / p.hk];
-  uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (slot >= 0 && slot < p.num_slots) {
-    const uint8_t* pg = (key ? p.k_cache : p.v_cache) + ((slot / PAGE) * p.hk + row % p.hk) * Geo<D>::PAGE_BYTES;
-    const int off = static_cast<int>(slot % PAGE);
-    const uint2 codes = *reinterpret_cast<const uint2*>(pg + off * Geo<D>::ROW + blk * 8);
-    __nv_fp8_e4m3 sc;
-    sc.__x = pg[PAGE * Geo<D>::ROW + off * Geo<D>::SROW + blk];
-    const float sf = static_cast<float>(sc), gs = key ? p.k_scale : p.v_scale;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t byte = ((j < 4 ? codes.x : codes.y) >> (8 * (j & 3))) & 0xff;
-      float v[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t c = (byte >> (4 * e)) & 15, m = c & 7;
-        // e2m1: 0, 0.5, then (1 + bit 0 / 2) 2^(bits 2..1 - 1)
-        const float mag = m < 2 ? 0.5f * m : __uint_as_float((126 + (m >> 1)) << 23 | (m & 1) << 22);
-        v[e] = (c & 8 ? -mag : mag) * sf * gs;
+  const int item = threadIdx.x % ITEMS, h0 = threadIdx.x % 32 / ITEMS;
+  const int half = p.rot / 2, pairs = half / 8;
+  const bool rotates = item < pairs;
+  const int unit = rotates ? item : item + pairs, other = rotates ? pairs : ITEMS - pairs;  // its second unit is unit + other
+  const int heads = p.hq + 2 * p.hk, all = (heads + STEP - 1) / STEP;
+  const int64_t runs = static_cast<int64_t>(gridDim.x) * (WRITE_THREADS / 32);
+  const int64_t run = static_cast<int64_t>(blockIdx.x) * (WRITE_THREADS / 32) + threadIdx.x / 32;
+  const int64_t total = p.num_tokens * all, first = run * total / runs;
+  const int count = static_cast<int>((run + 1) * total / runs - first);
+  if (count <= 0) return;
+
+  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(ring + threadIdx.x));
+  auto place = [](int s, int k) { return static_cast<uint32_t>((s * 6 + k) * WRITE_THREADS * 16); };
+  // where the copies are, and where the reads are
+  int64_t ft = first / all, ct = ft;
+  int fe = static_cast<int>(first - ft * all), ce = fe, asked = 0;
+  int64_t fpos = p.positions[ft], npos = ft + 1 < p.num_tokens ? p.positions[ft + 1] : 0;
+  bool fresh = true;  // the copies' token has no cosines yet
+  auto fetch = [&]() {
+    if (asked < count) {
+      const uint32_t to = base + place(asked % DEPTH, 0);
+      const int h = fe * STEP + h0;
+      if (h < heads) {
+        const __nv_bfloat16* src = p.qkv + ft * p.qkv_stride + static_cast<int64_t>(h) * D + unit * 8;
+        async16(to, src);
+        async16(to + place(0, 1), src + other * 8);
       }
-      const __nv_bfloat162 b = __floats2bfloat162_rn(v[0], v[1]);
-      w[j] = *reinterpret_cast<const uint32_t*>(&b);
+      if (fresh && rotates) {
+        const int64_t pos = fpos < 0 || fpos >= p.max_pos ? 0 : fpos;  // never past the table
+        const float* cs = p.cos_sin + pos * p.rot + item * 8;
+        async16(to + place(0, 2), cs);
+        async16(to + place(0, 3), cs + 4);
+        async16(to + place(0, 4), cs + half);
+        async16(to + place(0, 5), cs + half + 4);
+      }
+      fresh = false;
+      ++asked;
+      if (++fe == all) {
+        fe = 0;
+        ++ft;
+        fresh = true;
+        fpos = npos;
+        npos = ft + 1 < p.num_tokens ? p.positions[ft + 1] : 0;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int i = 0; i < DEPTH - 1; ++i) fetch();
+
+  int64_t slot = p.slots[ct], next_slot = ct + 1 < p.num_tokens ? p.slots[ct + 1] : 0;
+  float c[8], s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+  bool stale = true;
+#pragma unroll 1
+  for (int n = 0; n < count; ++n) {
+    fetch();
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+    const uint4* at = ring + (n % DEPTH) * 6 * WRITE_THREADS + threadIdx.x;
+    if (stale && rotates) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        *reinterpret_cast<uint4*>(c + 4 * i) = at[(2 + i) * WRITE_THREADS];
+        *reinterpret_cast<uint4*>(s + 4 * i) = at[(4 + i) * WRITE_THREADS];
+      }
+    }
+    stale = false;
+    const bool cached = slot >= 0 && slot < p.num_slots;
+    const int h = ce * STEP + h0;
+    const bool pages = cached && ce * STEP + STEP > p.hq;  // some of the step's heads go into the cache
+    if (h < p.hq || pages) {
+      float x[8], y[8];
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      unpack8(h < heads ? at[0] : zero, x);
+      unpack8(h < heads ? at[WRITE_THREADS] : zero, y);
+      if (rotates && h < p.hq + p.hk) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float u = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i]));
+          y[i] = __fadd_rn(__fmul_rn(y[i], c[i]), __fmul_rn(x[i], s[i]));
+          x[i] = u;
+        }
+      }
+      if (h < p.hq) {
+        uint4* dst = reinterpret_cast<uint4*>(p.q_out + ct * p.q_stride + static_cast<int64_t>(h) * D) + unit;
+        dst[0] = pack8(x);
+        dst[other] = pack8(y);
+      }
+      if (pages) {
+        const int j = h - p.hq;
+        const bool key = j < p.hk;
+        uint8_t* pg = (key ? p.k_cache : p.v_cache) + (slot / PAGE * p.hk + (key ? j : j - p.hk)) * Geo<D>::PAGE_BYTES;
+        const int off = static_cast<int>(slot % PAGE);
+        const float inv = key ? p.k_inv : p.v_inv;
+        const bool live = j >= 0 && h < heads;
+        put_unit<D>(pg, off, unit, x, inv, live);
+        put_unit<D>(pg, off, unit + other, y, inv, live);
+      }
+    }
+    if (++ce == all) {
+      ce = 0;
+      ++ct;
+      stale = true;
+      slot = next_slot;
+      next_slot = ct + 1 < p.num_tokens ? p.slots[ct + 1] : 0;
     }
   }
-  uint4* dst = reinterpret_cast<uint4*>((key ? p.k_out : p.v_out) + row * D + blk * 16);
-  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+// A thread reads READ_UNITS units of 8 dimensions, a CTA's in one run, in flight together.  Divisions by a slot's units
+// are done in 32 bits, within the CTA (in 64 bits for each thread they were most of the kernel's time).
+template <int D>
+__global__ void __launch_bounds__(READ_THREADS) read_kernel(KvFp4ReadParams p) {
+  constexpr int UNITS = D / 8;
+  shk::pdl_trigger();
+  shk::pdl_wait();
+  const bool key = blockIdx.y == 0;
+  const unsigned units = p.hk * UNITS;  // of a slot
+  const int64_t begin = static_cast<int64_t>(blockIdx.x) * (READ_THREADS * READ_UNITS);
+  const int64_t n0 = begin / units;
+  const unsigned r0 = static_cast<unsigned>(begin - n0 * units) + threadIdx.x;
+  const uint8_t* cache = key ? p.k_cache : p.v_cache;
+  const float gs = key ? p.k_scale : p.v_scale;
+  uint4* out = reinterpret_cast<uint4*>(key ? p.k_out : p.v_out) + begin + threadIdx.x;
+  const int64_t left = p.n * units - begin - threadIdx.x;
+  uint32_t codes[READ_UNITS] = {};
+  uint8_t sc[READ_UNITS] = {};
+#pragma unroll
+  for (int i = 0; i < READ_UNITS; ++i) {
+    if (i * READ_THREADS >= left) break;
+    const unsigned r = r0 + i * READ_THREADS, n = r / units, u = r - n * units;
+    const int64_t slot = p.slots[n0 + n];
+    if (slot < 0 || slot >= p.num_slots) continue;
+    const uint8_t* pg = cache + (slot / PAGE * p.hk + u / UNITS) * Geo<D>::PAGE_BYTES;
+    const int off = static_cast<int>(slot % PAGE), unit = u % UNITS;
+    codes[i] = *reinterpret_cast<const uint32_t*>(pg + off * Geo<D>::ROW + unit * 4);
+    sc[i] = pg[PAGE * Geo<D>::ROW + off * Geo<D>::SROW + (unit >> 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < READ_UNITS; ++i) {
+    if (i * READ_THREADS >= left) break;
+    __nv_fp8_e4m3 e;
+    e.__x = sc[i];
+    const float sf = static_cast<float>(e);
+    uint32_t w[4];
+    asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+        " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
+        : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+        : "r"(codes[i]));
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+      x[2 * k] = v.x * sf * gs;
+      x[2 * k + 1] = v.y * sf * gs;
+    }
+    out[i * READ_THREADS] = pack8(x);
+  }
 }
 
 // Page copies in every tensor: a CTA moves up to 16 KB of one page, four 16-byte loads a thread in flight.
@@ -238,16 +440,38 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_kernel(const __grid_constan
 using namespace shk::kv4;
 
 namespace {
-template <int D, int TPT>
+template <int D, int TPT, bool WHOLE>
 cudaError_t launch_write(const KvFp4WriteParams& p, cudaStream_t stream) {
   constexpr int TOKENS = WRITE_THREADS / TPT;
-  const dim3 grid(static_cast<unsigned>((p.num_tokens + TOKENS - 1) / TOKENS)), block(WRITE_THREADS);
-  return p.rot % 32 == 0 ? shk::launch(write_kernel<D, TPT, true>, grid, block, 0, stream, p)
-                         : shk::launch(write_kernel<D, TPT, false>, grid, block, 0, stream, p);
+  const dim3 grid(static_cast<unsigned>((p.num_tokens + TOKENS - 1) / TOKENS));
+  return shk::launch(write_kernel<D, TPT, WHOLE>, grid, dim3(WRITE_THREADS), 0, stream, p);
+}
+template <int D>
+cudaError_t launch_stream(const KvFp4WriteParams& p, cudaStream_t stream) {
+  constexpr int kMaxDevices = 64;
+  constexpr size_t smem = static_cast<size_t>(DEPTH) * 6 * WRITE_THREADS * 16;
+  static int sms[kMaxDevices];  // 0: this device has not been set up
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  if (!sms[dev]) {
+    int n = 0;
+    if ((e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    if ((e = cudaFuncSetAttribute(write_stream_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>(smem))) != cudaSuccess)
+      return e;
+    sms[dev] = n;
+  }
+  return shk::launch(write_stream_kernel<D>, dim3(sms[dev] * STREAM_CTAS), dim3(WRITE_THREADS), smem, stream, p);
 }
 template <int D>
 cudaError_t launch_write(const KvFp4WriteParams& p, cudaStream_t stream) {
-  return p.num_tokens < kFewTokens ? launch_write<D, 256>(p, stream) : launch_write<D, 32>(p, stream);
+  // a table that does not start on 16 bytes is read singly
+  const bool whole = p.rot % 32 == 0 && !(reinterpret_cast<uintptr_t>(p.cos_sin) & 15);
+  const bool few = p.num_tokens < kFewTokens;
+  if (whole) return few ? launch_write<D, 256, true>(p, stream) : launch_stream<D>(p, stream);
+  return few ? launch_write<D, 256, false>(p, stream) : launch_write<D, 32, false>(p, stream);
 }
 }  // namespace
 
@@ -271,9 +495,10 @@ extern "C" int sh_kv_fp4_write(const KvFp4WriteParams* params, int head_dim, cud
 extern "C" int sh_kv_fp4_read(const KvFp4ReadParams* params, int head_dim, cudaStream_t stream) {
   const KvFp4ReadParams& p = *params;
   if (p.n <= 0) return 0;
-  const int64_t ctas = (p.n * p.hk * (head_dim / 16) + 255) / 256;
+  constexpr int64_t per = READ_THREADS * READ_UNITS;
+  const int64_t ctas = (p.n * p.hk * (head_dim / 8) + per - 1) / per;
   if (ctas > 0x7fffffff) return -1;
-  const dim3 grid(static_cast<unsigned>(ctas), 2), block(256);
+  const dim3 grid(static_cast<unsigned>(ctas), 2), block(READ_THREADS);
   cudaError_t e;
   switch (head_dim) {
     case 64: e = shk::launch(read_kernel<64>, grid, block, 0, stream, p); break;

@@ -351,6 +351,65 @@ def test_write_extremes():
     assert (kr[0] == 0).all() and (kr[3] == 2688).all()
 
 
+@pytest.mark.parametrize("hq,hk,d,rot", [(32, 8, 128, 128), (16, 2, 256, 64), (4, 2, 64, 64), (7, 1, 128, 96), (3, 3, 64, 0),
+                                         (5, 3, 256, 256), (4, 1, 256, 0), (1, 5, 128, 32), (4, 2, 128, 24)])
+@pytest.mark.parametrize("T", [599, 1199, 2503])
+def test_write_many_tokens(hq, hk, d, rot, T):
+    """Tokens that share warps, some of them not cached, positions outside the table, and rows of any stride."""
+    qkv, pos, cs, slots, k, v = write_case(T, hq, hk, d, rot, seed=T + d, pad=8 * (hq % 2))
+    slots[::7], slots[5], slots[T - 1] = -1, 1 << 40, -(1 << 40)
+    pos[11], pos[12] = -3, 512
+    want_pos = torch.where((pos < 0) | (pos >= 512), 0, pos)  # positions outside the table read its first row
+    kd, vd = k.cuda(), v.cuda()
+    q = ops.rope_kv_write_fp4(qkv.cuda(), pos.cuda(), cs.cuda(), kd, vd, slots.cuda(), hq, hk, d, rot, 0.75, 2.0)
+    want = ops.rope_kv_write_fp4(qkv, want_pos, cs, k, v, slots, hq, hk, d, rot, 0.75, 2.0)
+    assert torch.equal(q.cpu(), want)
+    assert torch.equal(kd.cpu(), k) and torch.equal(vd.cpu(), v)
+    kr, vr = ops.kv_fp4_read(kd, vd, slots.cuda(), d, 0.75, 2.0)
+    kw, vw = ops.kv_fp4_read(k, v, slots, d, 0.75, 2.0)
+    assert torch.equal(kr.cpu(), kw.bfloat16()) and torch.equal(vr.cpu(), vw.bfloat16())
+
+
+@pytest.mark.parametrize("T", [40, 1280])
+def test_write_values_on_and_beside_the_ties(T):
+    """Every scale mantissa, values on each tie between two codes and the nearest bf16 values on both sides of it."""
+    hq, hk, d = 2, 1, 128
+    qkv, pos, cs, slots, k, v = write_case(T, hq, hk, d, 0, seed=6)
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    for t in range(T):
+        for b in range(8):
+            s = (8 + b) / 8.0 * 2.0 ** (t % 40 - 20 if t % 40 > 14 else t % 40 - 6)
+            s = max(s, 2.0 ** -8)
+            tie = (ties * s).bfloat16()
+            beside = torch.cat((tie.view(torch.int16) + 1, tie.view(torch.int16) - 1)).view(torch.bfloat16)
+            x = torch.cat((tie, beside))[torch.randperm(21, generator=torch.Generator().manual_seed(t * 8 + b))[:15]]
+            x = torch.cat((torch.tensor([6.0 * s]).bfloat16(), x)) * (1 if t % 2 else -1)
+            qkv[t, hq * d + 16 * b: hq * d + 16 * b + 16] = x
+            qkv[t, (hq + 1) * d + 16 * b: (hq + 1) * d + 16 * b + 16] = x.flip(0)
+    kd, vd = k.cuda(), v.cuda()
+    ops.rope_kv_write_fp4(qkv.cuda(), pos.cuda(), cs.cuda(), kd, vd, slots.cuda(), hq, hk, d, 0, 1.0, 0.5)
+    ops.rope_kv_write_fp4(qkv, pos, cs, k, v, slots, hq, hk, d, 0, 1.0, 0.5)
+    assert torch.equal(kd.cpu(), k) and torch.equal(vd.cpu(), v)
+
+
+@pytest.mark.parametrize("T", [3, 1300])
+def test_write_extremes_and_an_odd_table_start(T):
+    """Infinities and NaN in some blocks only; a cosine table that starts on 4 bytes."""
+    hq, hk, d = 2, 2, 128
+    qkv, pos, cs, slots, k, v = write_case(T, hq, hk, d, 64, seed=8)
+    qkv[::3, 5::16] = math.inf
+    qkv[1::3, 9::32] = -math.inf
+    qkv[2::3, 700::40] = math.nan
+    buf = torch.zeros(cs.numel() + 1, device="cuda")
+    buf[1:] = cs.flatten().cuda()
+    odd = buf[1:].view(cs.shape)
+    kd, vd = k.cuda(), v.cuda()
+    q = ops.rope_kv_write_fp4(qkv.cuda(), pos.cuda(), odd, kd, vd, slots.cuda(), hq, hk, d, 64)
+    want = ops.rope_kv_write_fp4(qkv, pos, cs, k, v, slots, hq, hk, d, 64)
+    assert torch.equal(q.cpu().isnan(), want.isnan()) and torch.equal(q.cpu().nan_to_num(), want.nan_to_num())
+    assert torch.equal(kd.cpu(), k) and torch.equal(vd.cpu(), v)
+
+
 def test_write_refusals():
     qkv, pos, cs, slots, k, v = (t.cuda() for t in write_case(4, 4, 2, 64, 64))
 
