@@ -224,7 +224,7 @@ __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, const Reque
     }
     while (c.tile >= c.r.tiles) {
       ++c.b;
-      c.r = c.b - table_b < kTable ? table[c.b - table_b] : request(p, c.b, ROWS);
+      c.r = table != nullptr && c.b - table_b < kTable ? table[c.b - table_b] : request(p, c.b, ROWS);
       c.tile = 0;
     }
     s.u0 = c.next;
@@ -277,6 +277,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   using K = Cfg<D, NT>;
   constexpr int ROWS = 8 * NT, WARPS = K::WARPS, THREADS = K::THREADS, STAGES = K::STAGES;
   constexpr int CHUNK = K::CHUNK, SUB = K::SUB;
+  constexpr int SCOUT = THREADS - 32;  // the thread that walks the run's units, in a warp that has no queries to convert
   constexpr int MT = D / 16;  // M tiles of O^T
   constexpr int KW = D / 32;  // words of a key in a thread (D/4 codes), two k-steps each
   constexpr int VW = D / 64;  // words of a value in a thread (D/8 codes), four M tiles each
@@ -287,13 +288,13 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   float* merge_l = merge_m + WARPS * ROWS;
   float* row_scale2 = merge_l + WARPS * ROWS;                      // [2][ROWS]
   int* row_pos2 = reinterpret_cast<int*>(row_scale2 + 2 * ROWS);  // [2][ROWS] last key a row sees
-  __shared__ int64_t scan[WARPS + 1];
-  __shared__ int64_t start_base;
+  __shared__ int64_t scan[WARPS];
   __shared__ int start_b;
   __shared__ Request table[kTable];  // of requests start_b, start_b + 1, ...
   __shared__ Cursor cursor;
-  __shared__ Segment segs[3];  // this unit, the next one and the one behind it, found by thread 0
-  __shared__ int seg_ok[3];
+  // this unit, the next one and the one behind it; the one before may still be read when that one is written
+  __shared__ Segment segs[4];
+  __shared__ int seg_ok[4];
   __shared__ Segment open[2];  // units that this CTA has a partial of: at most the run's first and last
   __shared__ int last_flag[2];
 
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
     first_w = weight(p, mine);
   }
   for (int b = threadIdx.x + THREADS; b < p.B; b += THREADS) rest += weight(p, request(p, b, ROWS));
-  auto scan_warps = [&](int64_t w) {  // inclusive over the block; the block's sum goes to scan[WARPS]
+  auto scan_warps = [&](int64_t w, int64_t& all) {  // inclusive over the block; a barrier lies between two calls
     int64_t incl = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -321,74 +322,59 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    int64_t before = 0, all = 0;
+    int64_t before = 0;
+    all = 0;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) {
       before += i < warp ? scan[i] : 0;
       all += scan[i];
     }
-    __syncthreads();
-    if (threadIdx.x == 0) scan[WARPS] = all;
     return before + incl;
   };
-  int64_t total = 0;
+  int64_t total = 0, done;
   if (p.B > THREADS) {
-    (void)scan_warps(rest);
+    (void)scan_warps(rest, total);
     __syncthreads();
-    total = scan[WARPS];
   }
-  int64_t incl = scan_warps(first_w);
-  __syncthreads();
-  int64_t done = scan[WARPS];
+  int64_t incl = scan_warps(first_w, done);
   total += done;
   int64_t per = quotient(total + gridDim.x - 1, gridDim.x);
   if (per < K::MIN_PAGES) per = K::MIN_PAGES;
   const int64_t run = per * blockIdx.x;
   if (run >= total) return;
-  if (incl - first_w <= run && run < incl) {
-    start_b = threadIdx.x;
-    start_base = incl - first_w;
-  }
-  for (int64_t b0 = THREADS; done <= run; b0 += THREADS) {
-    const int64_t b = b0 + threadIdx.x;
-    const int64_t w = b < p.B ? weight(p, request(p, static_cast<int>(b), ROWS)) : 0;
-    incl = done + scan_warps(w);
-    if (incl - w <= run && run < incl) {
-      start_b = static_cast<int>(b);
-      start_base = incl - w;
-    }
-    __syncthreads();
-    done += scan[WARPS];
-    __syncthreads();
-  }
-  __syncthreads();
-  {
-    const int i = static_cast<int>(threadIdx.x) - start_b;  // start_b + i is this thread's request, if it is among the first
-    if (i >= 0 && i < kTable && threadIdx.x < p.B) table[i] = mine;
-    if (start_b + kTable > THREADS && threadIdx.x < kTable && start_b + threadIdx.x >= THREADS && start_b + threadIdx.x < p.B)
-      table[threadIdx.x] = request(p, start_b + threadIdx.x, ROWS);
-  }
-  __syncthreads();
-  auto advance = [&](int slot) {  // thread 0: the next unit of the run
-    Cursor c = cursor;
+  auto advance = [&](Cursor c, const Request* known, int slot) {  // one thread: the next unit of the run
     Segment sg;
-    seg_ok[slot] = next_segment<ROWS, CHUNK, K::MIN_PAGES>(p, table, start_b, c, sg);
+    seg_ok[slot] = next_segment<ROWS, CHUNK, K::MIN_PAGES>(p, known, start_b, c, sg);
     segs[slot] = sg;
     cursor = c;
   };
-  if (threadIdx.x == 0) {  // the unit that the run begins in; the cursor stands before it
+  // The thread whose request the run begins in goes to its first unit at once.
+  auto take = [&](int b, const Request& r, int64_t base) {
+    start_b = b;
     Cursor c;
     c.pos = run;
     c.end = run + per < total ? run + per : total;
-    c.r = table[0];
-    const int64_t unit = quotient(run - start_base, c.r.pages + kUnit);
-    c.b = start_b;
+    c.r = r;
+    const int64_t unit = quotient(run - base, r.pages + kUnit);
+    c.b = b;
     c.tile = static_cast<int>(quotient(unit, p.hk));
-    c.h = static_cast<int>(unit - static_cast<int64_t>(c.tile) * p.hk) - 1;
-    c.next = start_base + unit * (c.r.pages + kUnit);
-    cursor = c;
-    advance(0);
-    advance(1);
+    c.h = static_cast<int>(unit - static_cast<int64_t>(c.tile) * p.hk) - 1;  // the cursor stands before it
+    c.next = base + unit * (r.pages + kUnit);
+    advance(c, nullptr, 0);
+  };
+  if (incl - first_w <= run && run < incl) take(threadIdx.x, mine, incl - first_w);
+  for (int64_t b0 = THREADS; done <= run; b0 += THREADS) {
+    __syncthreads();
+    const int64_t b = b0 + threadIdx.x;
+    Request other = {};
+    int64_t w = 0, all;
+    if (b < p.B) {
+      other = request(p, static_cast<int>(b), ROWS);
+      w = weight(p, other);
+    }
+    incl = done + scan_warps(w, all);
+    if (incl - w <= run && run < incl) take(static_cast<int>(b), other, incl - w);
+    done += all;
   }
   __syncthreads();
 
@@ -496,17 +482,29 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       }
     }
   };
+  Rows first = {};
   if (seg_ok[0]) {
-    const Rows x = load_rows(segs[0]);
+    first = load_rows(segs[0]);
     begin(segs[0]);  // the first keys are on their way before the queries are looked at
-    fetch();
-    convert(segs[0], 0, x);
+    do fetch();
+    while (asked < STAGES - 1 && pc < pc1);
+  }
+  {
+    const int i = static_cast<int>(threadIdx.x) - start_b;  // start_b + i is this thread's request, if it is among the first
+    if (i >= 0 && i < kTable && threadIdx.x < p.B) table[i] = mine;
+    if (start_b + kTable > THREADS && threadIdx.x < kTable && start_b + threadIdx.x >= THREADS && start_b + threadIdx.x < p.B)
+      table[threadIdx.x] = request(p, start_b + threadIdx.x, ROWS);
   }
   __syncthreads();
-  for (; seg_ok[unit % 3]; ++unit) {
-    const Segment& s = segs[unit % 3];
-    const Segment& sn = segs[(unit + 1) % 3];
-    const bool have = seg_ok[(unit + 1) % 3];
+  if (seg_ok[0]) {
+    if (threadIdx.x == SCOUT) advance(cursor, table, 1);
+    convert(segs[0], 0, first);
+  }
+  __syncthreads();
+  for (; seg_ok[unit % 4]; ++unit) {
+    const Segment& s = segs[unit % 4];
+    const Segment& sn = segs[(unit + 1) % 4];
+    const bool have = seg_ok[(unit + 1) % 4];
     const int turn = unit & 1, c_end = s.c1, kv_end = s.kv_end;
     const uint4* query = query2 + turn * NT * KW * 32;
     const float* row_scale = row_scale2 + turn * ROWS;
@@ -750,8 +748,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
 
     // (the barriers below stand before the use of both)
     if (have) convert(sn, turn ^ 1, load_rows(sn));
-    if (threadIdx.x == 0 && have) advance((unit + 2) % 3);
-    else if (threadIdx.x == 0) seg_ok[(unit + 2) % 3] = 0;
+    if (threadIdx.x == SCOUT) {
+      if (have) advance(cursor, table, (unit + 2) % 4);
+      else seg_ok[(unit + 2) % 4] = 0;
+    }
     // -------------------------------------------------------------- the warps' states become one
     if constexpr (K::SHARED) {  // no copy may land in the merge area
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -851,9 +851,6 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
       float top = -FLT_MAX, sum = 0.f, acc[DT];
 #pragma unroll
       for (int k = 0; k < DT; ++k) acc[k] = 0.f;
-      for (int c = first + lane; c <= last; c += 32) top = fmaxf(top, __ldcg(at(c) + ROWS * D + 2 * row));
-#pragma unroll
-      for (int o2 = 16; o2 > 0; o2 >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
       for (int c0 = first; c0 <= last; c0 += BATCH) {
         float2 ml[BATCH], v[BATCH][DT / 2];
 #pragma unroll
@@ -863,6 +860,14 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
 #pragma unroll
           for (int k = 0; k < DT / 2; ++k) v[b][k] = __ldcg(reinterpret_cast<const float2*>(src + row * D + lane * DT + 2 * k));
         }
+        float to = top;
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) to = fmaxf(to, ml[b].x);
+        const float al = ex2(top - to);  // the batches before, on the new reference
+        top = to;
+        sum *= al;
+#pragma unroll
+        for (int k = 0; k < DT; ++k) acc[k] *= al;
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
           if (c0 + b > last) break;
