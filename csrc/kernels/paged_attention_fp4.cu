@@ -26,6 +26,12 @@
 // The softmax keeps, per row, a reference m that moves only when a score exceeds it by more than 8 (in log2 units):
 // P <= 2^8 stays far from f16's range, and a chunk costs one vote instead of a reduction over the tokens.
 //
+// What bounds it.  Many keys and 8 rows: memory, behind the decoding (8 requests of 131072 keys, 32 heads of 128, 8 kv
+// heads: 1.18 GB in 228 us, 79% of the copy rate).  Short runs: the way to the first key and the merges, about 10 us of
+// latency around 22 pages (64 requests of 2048: 115 MB in 37 us, 48%; 24 of 4000 at head_dim 256: 40 MB in 23 us, 27%).
+// Wide windows: 255 registers leave two warps a scheduler, which wait for their own results (32 windows of 6 tokens,
+// 24 rows: 233 MB in 96 us, 37%, 43% of the issue slots and 41% of the tensor pipe's cycles).
+//
 // Rows that see no key give 0.  Tokens past the end of a sequence are read (they lie in its last page) with V's
 // scale replaced by 0 and their scores by -inf, so what an earlier owner left there does not matter.
 #include <float.h>
