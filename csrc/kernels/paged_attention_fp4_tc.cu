@@ -47,9 +47,6 @@ using namespace shk::tc;
 
 constexpr int PAGE = 64;
 constexpr int KT = PAGE;  // keys per tile
-constexpr int PRODUCERS = 3;  // warps each for K and V
-constexpr int MMA_WARP = 8 + 2 * PRODUCERS;
-constexpr int THREADS = (MMA_WARP + 2) * 32;
 constexpr float kSlack = 8.f;
 constexpr int kMergeDims = 16;
 constexpr int kMinTiles = 4;  // shortest piece of a unit that is cut
@@ -59,6 +56,10 @@ template <int D>
 struct Smem {
   static constexpr int NQ = D == 256 ? 1 : 2;     // query tiles
   static constexpr int ROWS = 128 * NQ;           // query rows per unit
+  static constexpr int FIRST = 4 * NQ;            // first producer warp
+  static constexpr int PRODUCERS = NQ == 1 ? 4 : 3;   // warps each for K and V
+  static constexpr int MMA_WARP = FIRST + 2 * PRODUCERS;  // one for each query tile
+  static constexpr int THREADS = (MMA_WARP + NQ) * 32;
   static constexpr int STAGES = D == 256 ? 2 : 4;
   static constexpr int SLABS = D / 64;            // 64 dimensions: one 128-byte swizzle row
   static constexpr int QSLAB = 128 * 128;         // 128 rows of one slab
@@ -400,9 +401,9 @@ __device__ __forceinline__ uint4 decode8(uint32_t w, uint32_t s2) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p) {
+__global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p) {
   using M = Smem<D>;
-  constexpr int ROWS = M::ROWS, NQ = M::NQ, STAGES = M::STAGES;
+  constexpr int ROWS = M::ROWS, NQ = M::NQ, STAGES = M::STAGES, MMA_WARP = M::MMA_WARP;
   constexpr uint32_t T_S = 0, T_O = 256, T_COLS = 512;
   constexpr int PAGE_BYTES = PAGE * (D / 2 + D / 16);
   extern __shared__ uint8_t smem_raw[];
@@ -426,9 +427,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
       mbar_init(&drain[i], 1);
     }
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&kfull[i], PRODUCERS);
+      mbar_init(&kfull[i], M::PRODUCERS);
       mbar_init(&kempty[i], NQ);
-      mbar_init(&vfull[i], PRODUCERS);
+      mbar_init(&vfull[i], M::PRODUCERS);
       mbar_init(&vempty[i], NQ);
     }
     for (int i = 0; i < 4; ++i) {
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
   shk::pdl_wait();  // lengths, tables, queries and the new tokens' rows come from earlier kernels
 
   Cursor cur;
-  const int64_t per = find_run<ROWS, THREADS>(p, blockIdx.x, gridDim.x, cur);
+  const int64_t per = find_run<ROWS, M::THREADS>(p, blockIdx.x, gridDim.x, cur);
   if (threadIdx.x == 0) splits<D>(p, gridDim.x)[blockIdx.x].last = -1;
   fence_before();
   __syncthreads();
@@ -456,13 +457,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_fp4_tc_kernel(AttnFp4Params p
   const uint32_t tmem = *tmem_slot;
   Segment s = {};
 
-  if (warp >= 8 && warp < MMA_WARP) {
+  if (warp >= M::FIRST && warp < MMA_WARP) {
     // ------------------------------------------------------------------ producers
     // A thread decodes 16-byte pieces (32 dimensions of a key): piece i of a tile is dimensions 32 (i % PR) .. of
     // key i / PR, so a warp's loads are one run of memory.
-    constexpr int PR = D / 32, PIECES = KT * PR, STEP = PRODUCERS * 32, N = (PIECES + STEP - 1) / STEP;
-    const bool value = warp >= 8 + PRODUCERS;  // this warp's matrix
-    const int tid = threadIdx.x - (value ? 8 + PRODUCERS : 8) * 32;
+    constexpr int PR = D / 32, PIECES = KT * PR, STEP = M::PRODUCERS * 32, N = (PIECES + STEP - 1) / STEP;
+    const bool value = warp >= M::FIRST + M::PRODUCERS;  // this warp's matrix
+    const int tid = threadIdx.x - (M::FIRST + (value ? M::PRODUCERS : 0)) * 32;
     const uint8_t* cache = value ? p.v_cache : p.k_cache;
     struct Codes {
       uint4 w[N];
@@ -930,7 +931,7 @@ int launch(const AttnFp4Params& p, cudaStream_t st) {
   }
   const int ctas = num_sms();
   if (ctas <= 0) return -5;
-  cudaError_t e = shk::launch(k, dim3(ctas), dim3(THREADS), Smem<D>::TOTAL, st, p);
+  cudaError_t e = shk::launch(k, dim3(ctas), dim3(Smem<D>::THREADS), Smem<D>::TOTAL, st, p);
   if (e == cudaSuccess) e = shk::launch(merge_kernel<D>, dim3(ctas, Smem<D>::NQ * D / kMergeDims), dim3(128), 0, st, p, ctas);
   return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
 }
