@@ -637,12 +637,12 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
     // through the last, so a parity is never two phases old.
     int ns = 0;
     bool ok = true;
-    // This thread's row of a unit: where it comes from and goes to, its scales, the last key it sees.
+    // This thread's row of a unit: where it comes from and goes to, its scale, the last key it sees.
     struct Row {
       const uint4* src;
       __nv_bfloat16* dst;
       int64_t pos;
-      float f, cs;
+      float cs;
       bool valid;
     };
     auto advance = [&](Segment& sg) {  // the next unit in which this query tile has rows
@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
       } while (more && (q * 128 >= sg.rows || sg.none));
       return more;
     };
-    auto scan_row = [&](const Segment& sg) {
+    auto row_of = [&](const Segment& sg) {
       Row w;
       const int n = q * 128 + r, rr = sg.row0 + n;
       const int64_t tok = sg.qs + rr / group, col = static_cast<int64_t>(sg.h * group + rr % group) * D;
@@ -660,35 +660,49 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
       w.src = reinterpret_cast<const uint4*>(p.q + tok * p.q_stride + col);
       w.dst = p.out + tok * p.out_stride + col;
       w.pos = sg.ctx0 + rr / group;
-      uint32_t top = 0;
-      if (w.valid) {
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint4 v = w.src[i];
-          const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) top = max(top, max(w4[k] & 0x7fffu, (w4[k] >> 16) & 0x7fffu));
-        }
-      }
-      // its largest element goes into [2^13, 2^14); the softmax scale's sign goes with the row (0: a zero row), so that
-      // cs > 0 and the largest S is the largest score
-      const int e = min(267 - static_cast<int>(top >> 7), 253);
-      w.f = p.scale_log2 == 0.f ? 0.f : copysignf(__uint_as_float(static_cast<uint32_t>(e) << 23), p.scale_log2);
-      w.cs = fmaxf(__uint_as_float(static_cast<uint32_t>(254 - e) << 23) * fabsf(p.scale_log2), FLT_MIN);
+      w.cs = 0.f;
       return w;
     };
-    auto store_row = [&](const Row& w) {
-      uint8_t* qrow = smem + M::Q + q * M::QTILE + r * 128;
+    // A warp's 32 rows, scaled and in f16, into their tile.  A row is read by D / 8 lanes (read by its own thread alone,
+    // each access touched 32 lines, and a unit waited 8 us for its queries).
+    auto load_rows = [&](Row& w) {
+      constexpr int LANES = D / 8, AT_ONCE = 32 / LANES, BATCH = 8;
+      uint8_t* tile = smem + M::Q + q * M::QTILE + (warp & 3) * 32 * 128;
+      const int i = lane % LANES;
+      const uint64_t from = w.valid ? reinterpret_cast<uint64_t>(w.src) : 0;
+      int own = 0;  // the exponent of this thread's row
+#pragma unroll 1
+      for (int b = 0; b < LANES; b += BATCH) {
+        uint4 v[BATCH];
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const uint4 v = w.valid ? w.src[i] : make_uint4(0, 0, 0, 0);  // the scan has left it in L1
-        const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
-        uint32_t o[4];
+        for (int k = 0; k < BATCH; ++k) {
+          const uint4* row = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, from, (b + k) * AT_ONCE + lane / LANES));
+          v[k] = row != nullptr ? row[i] : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          o[k] = pack_f16(__uint_as_float(w4[k] << 16) * w.f, __uint_as_float(w4[k] & 0xffff0000u) * w.f);
-        *reinterpret_cast<uint4*>(qrow + (i >> 3) * M::QSLAB + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int k = 0; k < BATCH; ++k) {
+          const int n = (b + k) * AT_ONCE + lane / LANES;
+          const uint32_t w4[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          uint32_t top = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = max(top, max(w4[j] & 0x7fffu, (w4[j] >> 16) & 0x7fffu));
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          // its largest element goes into [2^13, 2^14); the softmax scale's sign goes with the row (0: a zero row), so
+          // that cs > 0 and the largest S is the largest score
+          const int e = min(267 - static_cast<int>(top >> 7), 253);
+          const float f = p.scale_log2 == 0.f ? 0.f : copysignf(__uint_as_float(static_cast<uint32_t>(e) << 23), p.scale_log2);
+          const int there = __shfl_sync(0xffffffffu, e, lane % AT_ONCE * LANES);
+          if (lane / AT_ONCE == b + k) own = there;
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[j] = pack_f16(__uint_as_float(w4[j] << 16) * f, __uint_as_float(w4[j] & 0xffff0000u) * f);
+          *reinterpret_cast<uint4*>(tile + n * 128 + (i >> 3) * M::QSLAB + (((i & 7) ^ (n & 7)) << 4)) =
+              make_uint4(o[0], o[1], o[2], o[3]);
+        }
       }
+      w.cs = fmaxf(__uint_as_float(static_cast<uint32_t>(254 - own) << 23) * fabsf(p.scale_log2), FLT_MIN);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&qfull[q]);
@@ -696,15 +710,15 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
     Segment sn;
     bool have = advance(sn), stored = false;
     Row next = {};
-    if (have) next = scan_row(sn);
+    if (have) next = row_of(sn);
     while (have) {
       s = sn;
-      const Row w = next;
-      const float cs = w.cs;
       float m = -FLT_MAX, l = 0.f;
       const bool keys = s.k0 < s.k1;
+      if (keys && ok && !stored) load_rows(next);
+      const Row w = next;
+      const float cs = w.cs;
       if (keys && ok) {
-        if (!stored) store_row(w);
         // key tiles from here on hold keys that some row of this query tile does not see
         const int64_t seen = s.ctx0 + (s.row0 + q * 128) / group + 1;
         const int free_tiles = seen > 0 ? static_cast<int>(seen / KT) : 0;
@@ -786,18 +800,17 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
           if (lane == 0) mbar_arrive(&pfull[buf]);
         }
       }
-      // the next unit's row is read while this unit's last product runs, and stored for its MMAs before this one's
-      // results are written
+      // the next unit's rows take the place of this one's, whose last S has been seen, under its last product
       have = advance(sn);
-      if (have) next = scan_row(sn);
+      if (have) next = row_of(sn);
+      stored = have && ok && sn.k0 < sn.k1;
+      if (stored) load_rows(next);
       if (keys) {
         if (ok && !__all_sync(0xffffffffu, mbar_wait(&pvdone[q * 2 + ((ns - 1) & 1)], ((ns - 1) >> 1) & 1, abort_flag)))
           ok = false;
         if (!ok) *abort_flag = 1;
         fence_after();
       }
-      stored = have && ok && sn.k0 < sn.k1;
-      if (stored) store_row(next);
       if (!ok) l = __uint_as_float(0x7fc00000u);  // a wait ran out: NaN, not numbers
       const bool none = !keys || !ok;
       if (s.whole) {
