@@ -206,19 +206,20 @@ void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const
   const int64_t rows = std::min<int64_t>(max_q_len, 4096) * (hq / hk);  // of one kv head
   int r;
   // The tensor-core kernel takes units of 256 rows (128 at head_dim 256) whatever they hold, and starts up in 10 to
-  // 25 us; the other one's time grows with its row tiles, and a lone request's keys are spread over fewer warps.  Short
+  // 20 us; the other one's time grows with its row tiles, and a lone request's keys are spread over fewer warps.  Short
   // kernel against this one, in us:
-  //   rows: 32 requests of 6000 keys on average, head_dim 128, 107 against 174 at 32 rows, 181 against 175 at 36;
-  //     24 of 3000 at head_dim 256, 51 against 68 at 48, 61 against 69 at 64, 71 against 68 at 72;
-  //   keys, one request with 32 heads of 128: 12 against 23 for a prompt of 200, 34 against 24 for one of 300, 30 against
-  //     22 for 16 tokens at 1000, 83 against 57 for 17 at 30000;
-  //   work (query rows times keys at most), one request, 16 heads of 256: 18 against 26 for a prompt of 160 (0.5M), 33
-  //     against 35 for 400 (3M), 127 against 59 for 1000 (16M); 8 heads of 64: 10 against 19 for 400 (1.4M), 34 against
-  //     40 for 64 tokens at 12000 (6M), 33 against 23 for 1000 (8M).
+  //   rows: 32 requests of 6000 keys on average, head_dim 128, 100 against 172 at 32 rows, 173 against 173 at 36 and 48;
+  //     24 of 3000 at head_dim 256, 48 against 49 at 48, 58 against 49 at 64, 67 against 49 at 72;
+  //   keys, one request with 32 heads of 128: 12 against 21 for a prompt of 200, 29 against 21 for one of 300, 27 against
+  //     21 for 16 tokens at 1000, 80 against 54 for 17 at 30000;
+  //   work (query rows times keys at most), one request, 16 heads of 256: 17 against 20 for a prompt of 160 (0.5M), 32
+  //     against 39 for 17 tokens at 8000 (2.2M), 32 against 25 for a prompt of 400 (2.9M), 121 against 42 for one of 1000
+  //     (16M); 8 heads of 64: 10 against 18 for 400 (1.4M), 29 against 39 for 64 tokens at 12000 (6.2M), 31 against 22 for
+  //     1000 (8.2M).
   const int64_t keys = 64 * p.bt_cols;
   const double work = static_cast<double>(q.size(0)) * static_cast<double>(hq) * static_cast<double>(keys);
-  const bool large = work > 4e6 || (d == 128 && keys > 256);
-  if (rows > (d == 256 ? 64 : 32) && large && !invariant) {
+  const bool large = d == 128 ? keys > 256 || work > 4e6 : work > (d == 256 ? 2.5e6 : 7.5e6);
+  if (rows > (d == 256 ? 48 : 32) && large && !invariant) {
     const int64_t floats = sh_paged_attention_fp4_tc_workspace(dim);
     TORCH_CHECK(floats > 0, who, ": no CUDA device");
     const Scratch s = scratch(k_cache, stream, floats, 0);

@@ -8,16 +8,17 @@
 // unit cut by a run's end leaves fp32 partials, which a second kernel merges in order.  (The last CTA of a unit doing
 // it alone, as the short-query kernel does, pulls 133 KB per partial through one SM: 64 tokens over 20000 took 101 us.)
 //
-// Per CTA (512 threads):
-//   warps 0-3, 4-7   one warpgroup per query tile, a row a thread (= its TMEM lane): load the row, scale it by a power
-//                    of two into f16's range and store it for the MMA; per key tile read S, softmax in the exp2 domain
-//                    against a reference that moves only when a score passes it by more than 8, write P (f16) over S;
-//                    at the end O / l, or the partial;
-//   warps 8-10, 11-13 decode 64-key tiles (a page's head) of K and of V into f16 tiles (exact) in shared memory; the
-//                    next two tiles' codes are on their way in registers;
-//   warps 14, 15     issue the MMAs of a query tile each: S_q = Q_q K^T into one of two buffers, O_q += P_q V.  S of the next tile is
-//                    issued before P of this one is waited for, so the softmax never waits for a product it could have
-//                    had, and the products run under the other tile's (or buffer's) softmax.
+// Per CTA (16 warps; 13 at head_dim 256):
+//   4 NQ warps       a warpgroup per query tile: load its rows, scale each by a power of two into f16's range and store
+//                    it for the MMA; then a row a thread (= its TMEM lane): per key tile read S, softmax in the exp2
+//                    domain against a reference that moves only when a score passes it by more than 8, write P (f16)
+//                    over S; at the end O / l, or the partial;
+//   3 + 3 (4 + 4)    decode 64-key tiles (a page's head) of K and of V into f16 tiles (exact) in shared memory; the next
+//                    two tiles' codes are on their way in registers (head_dim 256 with 3 + 3: a prompt of 4096 with 16
+//                    heads took 360 us, with 5 + 5 255, with 4 + 4, a whole number of pieces a thread, 240);
+//   NQ warps         issue the MMAs of a query tile each: S_q = Q_q K^T into one of two buffers, O_q += P_q V.  S of the
+//                    next tile is issued before P of this one is waited for, so the softmax never waits for a product
+//                    it could have had, and the products run under the other tile's (or buffer's) softmax.
 // TMEM: S_q,b (64 columns each, P in their first 32), O_q (D columns each) from column 256.
 //
 // What bounds it.  No single pipe: a prompt of 8192 with 32 heads of 128 takes 615 us (894 TFLOP/s, 54% of the rate of a
@@ -25,7 +26,9 @@
 // the tensor pipe's cycles and 37% of the special-function unit's.  Without the softmax the chunk would take 808 us,
 // without the decoding 1014: the chain S, weights, product of one query tile hides behind the other's only in part.
 // Tried and slower: 128-key tiles with one S buffer, setmaxnreg splits (1110 us: the producers spill), a third tile's
-// codes in registers (1090), the tile's sum as the sign that the reference must move, in place of its maximum (1081).
+// codes in registers (1090), the tile's sum as the sign that the reference must move, in place of its maximum (1081), S
+// of two tiles in one product (1247, where the same code took 1079 with one).  A prompt of 4096 with 16 heads of 256 takes
+// 215 us (639 TFLOP/s, 38%): one query tile, whose softmax and products wait for each other.
 //
 // Every wait is bounded (2 s); one that runs out raises the CTA's abort flag, the rows of the CTA's units become NaN,
 // and the CTA drains its MMAs and frees its TMEM before it returns.
@@ -57,8 +60,8 @@ struct Smem {
   static constexpr int NQ = D == 256 ? 1 : 2;     // query tiles
   static constexpr int ROWS = 128 * NQ;           // query rows per unit
   static constexpr int FIRST = 4 * NQ;            // first producer warp
-  static constexpr int PRODUCERS = NQ == 1 ? 4 : 3;   // warps each for K and V
-  static constexpr int MMA_WARP = FIRST + 2 * PRODUCERS;  // one for each query tile
+  static constexpr int PRODUCERS = NQ == 1 ? 4 : 3;       // warps each for K and V
+  static constexpr int MMA_WARP = FIRST + 2 * PRODUCERS;  // and one for each query tile
   static constexpr int THREADS = (MMA_WARP + NQ) * 32;
   static constexpr int STAGES = D == 256 ? 2 : 4;
   static constexpr int SLABS = D / 64;            // 64 dimensions: one 128-byte swizzle row
@@ -686,8 +689,12 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
           uint32_t top = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) top = max(top, max(w4[j] & 0x7fffu, (w4[j] >> 16) & 0x7fffu));
+          if constexpr (LANES == 32) {
+            top = __reduce_max_sync(0xffffffffu, top);
+          } else {
 #pragma unroll
           for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          }
           // its largest element goes into [2^13, 2^14); the softmax scale's sign goes with the row (0: a zero row), so
           // that cs > 0 and the largest S is the largest score
           const int e = min(267 - static_cast<int>(top >> 7), 253);
