@@ -21,14 +21,16 @@
 //                    it could have had, and the products run under the other tile's (or buffer's) softmax.
 // TMEM: S_q,b (64 columns each, P in their first 32), O_q (D columns each) from column 256.
 //
-// What bounds it.  No single pipe: a prompt of 8192 with 32 heads of 128 takes 615 us (894 TFLOP/s, 54% of the rate of a
-// large bf16 product), a chunk of 2000 at 32768 keys 1020 us (1020 TFLOP/s, 61%), with 47% of the issue slots, 47% of
-// the tensor pipe's cycles and 37% of the special-function unit's.  Without the softmax the chunk would take 808 us,
-// without the decoding 1014: the chain S, weights, product of one query tile hides behind the other's only in part.
+// What bounds it.  No single pipe: a prompt of 8192 with 32 heads of 128 takes 595 us (924 TFLOP/s, 55% of the rate of a
+// large bf16 product), a chunk of 2000 at 32768 keys 995 us (1046 TFLOP/s, 63%), with about half of the issue slots, half
+// of the tensor pipe's cycles and 40% of the special-function unit's.  When the chunk took 1020, it took 808 without the
+// softmax and 1014 without the decoding: the chain S, weights, product of one query tile hides behind the other's only
+// in part.  Registers decide much: with the run's cursor in them, not in shared memory, the two took 615 and 1020.
 // Tried and slower: 128-key tiles with one S buffer, setmaxnreg splits (1110 us: the producers spill), a third tile's
 // codes in registers (1090), the tile's sum as the sign that the reference must move, in place of its maximum (1081), S
-// of two tiles in one product (1247, where the same code took 1079 with one).  A prompt of 4096 with 16 heads of 256 takes
-// 215 us (639 TFLOP/s, 38%): one query tile, whose softmax and products wait for each other.
+// of two tiles in one product (1247, where the same code took 1079 with one), results through shared memory (1078).  A
+// prompt of 4096 with 16 heads of 256 takes 207 us (664 TFLOP/s, 40%): one query tile, whose softmax and products wait
+// for each other.
 //
 // Every wait is bounded (2 s); one that runs out raises the CTA's abort flag, the rows of the CTA's units become NaN,
 // and the CTA drains its MMAs and frees its TMEM before it returns.
@@ -451,6 +453,7 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
   shk::pdl_trigger();
   shk::pdl_wait();  // lengths, tables, queries and the new tokens' rows come from earlier kernels
 
+  __shared__ Cursor saved[4 * NQ];
   Cursor cur;
   const int64_t per = find_run<ROWS, M::THREADS>(p, blockIdx.x, gridDim.x, cur);
   if (threadIdx.x == 0) splits<D>(p, gridDim.x)[blockIdx.x].last = -1;
@@ -650,9 +653,13 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
     };
     auto advance = [&](Segment& sg) {  // the next unit in which this query tile has rows
       bool more;
+      Cursor c = saved[warp];  // kept out of the registers, which the softmax needs
       do {
-        more = next_segment<ROWS>(p, cur, sg);
+        more = next_segment<ROWS>(p, c, sg);
       } while (more && (q * 128 >= sg.rows || sg.none));
+      __syncwarp();
+      if (lane == 0) saved[warp] = c;
+      __syncwarp();
       return more;
     };
     auto row_of = [&](const Segment& sg) {
@@ -714,6 +721,8 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
       __syncwarp();
       if (lane == 0) mbar_arrive(&qfull[q]);
     };
+    if (lane == 0) saved[warp] = cur;
+    __syncwarp();
     Segment sn;
     bool have = advance(sn), stored = false;
     Row next = {};
