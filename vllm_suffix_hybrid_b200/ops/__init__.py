@@ -189,8 +189,8 @@ def rope_kv_write_fp4(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, h
 
     qkv [T, (hq + 2 hk) D] is only read; the rotated queries [T, hq D] are returned (into q_out when given).  A row
     with a slot outside the cache (< 0: padding) caches nothing; of two rows with one slot either may be stored, in
-    parts.  The
-    caches hold x / k_scale and x / v_scale: e2m1 codes times e4m3 scales of 16 dimensions, from 2^-10 to 2688."""
+    parts.  The caches hold x / k_scale and x / v_scale: e2m1 codes times e4m3 scales of 16 dimensions, from 2^-10 to
+    2688."""
     rot = d if rot is None else rot
     if not _cuda(qkv):
         q = ref.rope_kv_write_fp4(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, hq, hk, d, rot, k_scale,
