@@ -3,10 +3,11 @@
 //
 // Work.  A unit is (request, kv head, NQ tiles of 128 packed query rows) that share every key tile, so a key is decoded
 // once per 256 rows (128 at head_dim 256, where two accumulators do not fit TMEM).  The units are laid end to end,
-// each as long as its share of the causal triangle (w_i = (ctx + c) G + (i + 1) ROWS for row tile i, c for a unit's
-// start and end: integers with a closed-form sum, so any place is found by bisection), and cut into one run per SM.  A
-// unit cut by a run's end leaves fp32 partials, which a second kernel merges in order.  (The last CTA of a unit doing
-// it alone, as the short-query kernel does, pulls 133 KB per partial through one SM: 64 tokens over 20000 took 101 us.)
+// each as long as its share of the causal triangle (w_i = (ctx + c) G + (i + 1) ROWS for row tile i, less the rows before
+// the first key, c for a unit's start and end: integers with a closed-form sum, so any place is found by bisection), and
+// cut into one run per SM.  A unit cut by a run's end leaves fp32 partials, which a second kernel merges in order.  (The
+// last CTA of a unit doing it alone, as the short-query kernel does, pulls 133 KB per partial through one SM: 64 tokens
+// over 20000 took 101 us.)
 //
 // Per CTA (16 warps; 13 at head_dim 256):
 //   4 NQ warps       a warpgroup per query tile: load its rows, scale each by a power of two into f16's range and store
@@ -219,7 +220,7 @@ __device__ __forceinline__ bool elect_one() {
 
 // What a request asks for, clipped to the tensors it indexes.
 struct Request {
-  int64_t qs, seq, ctx;  // ctx: tokens before the new ones, for the weights (never negative)
+  int64_t qs, seq, ctx;  // ctx: tokens before the new ones (negative: as many new ones come before the first key)
   int q_len, tiles;
 };
 template <int ROWS>
@@ -233,19 +234,23 @@ __device__ __forceinline__ Request request(const AttnFp4Params& p, int b) {
   if (r.seq < 0) r.seq = 0;
   const int64_t cap = static_cast<int64_t>(p.bt_cols) * PAGE;
   if (r.seq > cap) r.seq = cap;
-  r.ctx = r.seq > r.q_len ? r.seq - r.q_len : 0;
+  r.ctx = r.seq - r.q_len;
   r.tiles = static_cast<int>((static_cast<int64_t>(r.q_len) * (p.hq / p.hk) + ROWS - 1) / ROWS);
   return r;
 }
 // Cost of a request's row tile i, one kv head: the keys it sees (times the group) and kUnit keys for what a unit costs
-// besides; and of its first n tiles.
+// besides; and of its first n tiles.  Rows before the first key count for nothing: a cost that ran ahead of a unit's key
+// tiles would leave some run in the unit's middle without one, and the merge expects a partial of each.
 template <int ROWS>
 __device__ __forceinline__ int64_t tile_cost(const Request& r, int group, int64_t i) {
-  return (r.ctx + kUnit) * group + (i + 1) * ROWS;
+  const int64_t seen = r.ctx * group + (i + 1) * ROWS;
+  return kUnit * group + (seen > 0 ? seen : 0);
 }
 template <int ROWS>
 __device__ __forceinline__ int64_t cost(const Request& r, int group, int64_t n) {
-  return n * (r.ctx + kUnit) * group + ROWS * (n * (n + 1) / 2);
+  const int64_t a = r.ctx < 0 ? -r.ctx * group / ROWS : 0;  // tiles without a key
+  const int64_t seen = n > a ? (n - a) * r.ctx * group + ROWS * ((n * (n + 1) - a * (a + 1)) / 2) : 0;
+  return n * kUnit * group + seen;
 }
 
 // A unit of `tiles` key tiles and cost w, cut where `at` of w lies behind: the tile there, moved to an end of the unit
@@ -301,7 +306,7 @@ __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, 
   const int64_t left = static_cast<int64_t>(c.r.q_len) * g - s.row0;
   s.rows = left < ROWS ? static_cast<int>(left) : ROWS;
   s.qs = c.r.qs;
-  s.ctx0 = c.r.seq - c.r.q_len;
+  s.ctx0 = c.r.ctx;
   int64_t kv = s.ctx0 + (s.row0 + s.rows - 1) / g + 1;  // keys the tile's last row sees
   if (kv > c.r.seq) kv = c.r.seq;
   if (kv < 0) kv = 0;
@@ -342,7 +347,9 @@ __device__ __forceinline__ int64_t find_run(const AttnFp4Params& p, int run, int
   for (int w = 0; w < N / 32; ++w) total += scan[w];
   __syncthreads();
   int64_t per = (total + runs - 1) / runs;
-  const int64_t least = static_cast<int64_t>(kMinTiles) * KT * group;  // a run in the middle of a unit is never without a tile
+  // A run in the middle of a unit is never without a tile: a unit of kv keys costs at most (kv + kUnit) G + ROWS, so for
+  // the 9 tiles or more that leave cuts in its middle (kv > 512) a tile costs less than 2 KT G + ROWS / 9 < 4 KT G.
+  const int64_t least = static_cast<int64_t>(kMinTiles) * KT * group;
   if (per < least) per = least;
   cur.pos = per * run;
   cur.end = cur.pos + per < total ? cur.pos + per : total;
