@@ -51,16 +51,22 @@ void check_rows(const torch::Tensor& t, int64_t width, const torch::Tensor& like
 }
 
 // Partial results and tickets of the split units, one set per stream: calls on a stream follow one another, calls on
-// two streams may overlap.  A stream under capture gets a set of its own for that capture, so that a replay never
-// shares one with eager calls; it lives in the graph's pool, and its tickets are zeroed by a node of the graph.
+// two streams may overlap.  A capture has sets of its own, so that a replay never shares one with eager calls, and one for
+// each of its streams, for the branches of a graph may overlap too.  They live in the graph's pool; a set's tickets are
+// zeroed by a node of the graph, on the stream that the set belongs to.  The sets of a device's last capture are kept until
+// another one asks (one that is still open gets new ones then: the old memory is only reused behind its own stream's work).
 struct Scratch {
   torch::Tensor part, tickets;
+};
+struct CaptureScratch {
+  unsigned long long id = 0;
+  std::map<cudaStream_t, Scratch> sets;
 };
 
 Scratch scratch(const torch::Tensor& like, cudaStream_t stream, int64_t floats, int64_t ctas) {
   static std::mutex mu;
   static auto* eager = new std::map<std::pair<int, cudaStream_t>, Scratch>();  // never destroyed: outlives CUDA
-  static auto* captured = new std::map<int, std::pair<unsigned long long, Scratch>>();
+  static auto* captured = new std::map<int, CaptureScratch>();
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   unsigned long long id = 0;
   TORCH_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id) == cudaSuccess, "paged_attention_fp4: stream capture state");
@@ -68,9 +74,12 @@ Scratch scratch(const torch::Tensor& like, cudaStream_t stream, int64_t floats, 
   const int dev = like.get_device();
   Scratch* s;
   if (status == cudaStreamCaptureStatusActive) {
-    auto& slot = (*captured)[dev];
-    if (slot.first != id) slot = {id, Scratch{}};
-    s = &slot.second;
+    CaptureScratch& capture = (*captured)[dev];
+    if (capture.id != id) {
+      capture.sets.clear();
+      capture.id = id;
+    }
+    s = &capture.sets[stream];
   } else {
     s = &(*eager)[{dev, stream}];
   }

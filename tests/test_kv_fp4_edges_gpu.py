@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from test_kv_fp4_gpu import attend, case, check
+from vllm_suffix_hybrid_b200 import ops
 
 pytestmark = pytest.mark.gpu
 
@@ -21,3 +22,39 @@ def test_more_new_tokens_than_keys_over_many_runs(q, seq, hq, d):
     check(c, got)
     assert (got[: q - seq] == 0).all()
     assert torch.equal(got, attend(c))
+
+
+@pytest.mark.parametrize("shapes", [(((1,) * 5, (7000,) * 5), ((2,) * 4, (9000,) * 4)),
+                                    (((300,), (9000,)), ((90, 200), (5000, 700))), (((1,) * 5, (7000,) * 5), ((300,), (9000,)))])
+def test_branches_of_one_graph_do_not_disturb_each_other(shapes):
+    """Calls with cut units on two streams of one capture: each branch has partials and tickets of its own."""
+    cases = [case(q, s, 8, 2, 128, seed=50 + i) for i, (q, s) in enumerate(shapes)]
+    dev = [{n: c[n].cuda() for n in ("q", "k", "v", "bt", "seqs", "qs")} for c in cases]
+    outs = [torch.empty_like(d["q"]) for d in dev]
+
+    def call(i):
+        c, d = cases[i], dev[i]
+        for _ in range(3):
+            ops.paged_attention_fp4(outs[i], d["q"], d["k"], d["v"], d["bt"], d["seqs"], d["qs"], 8, 128, c["scale"],
+                                    c["max_q"], c["gk"], c["gv"])
+
+    want = []
+    for i in range(2):
+        call(i)
+        check(cases[i], outs[i])
+        want.append(outs[i].clone())
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call(1)
+        call(0)
+        torch.cuda.current_stream().wait_stream(side)
+    for _ in range(20):
+        for o in outs:
+            o.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
