@@ -542,6 +542,8 @@ class LLMEngine:
         # a long prompt's chunks alternate with decode steps of the running requests
         if self.prefilling is not None and (not self.running or self._last_kind != "chunk"):
             return self._chunk_step()
+        if self.waiting and not self.running and self.prefilling is None:
+            self._make_room()
         free_rows = self.cfg.max_num_seqs - len(self.running) - (self.prefilling is not None)
         # a waiting request is prefilled once a row is free and the KV blocks not promised to running requests
         # cover it (otherwise the running ones decode on, without breaking the decode pipeline, until they do)
@@ -611,6 +613,22 @@ class LLMEngine:
         if self.prefilling is not None:
             owed += self._missing(self.prefilling)
         return self.pool.free - owed
+
+    def _make_room(self) -> None:
+        """Nothing runs: if the first waiting request does not fit, forks that wait hold the blocks it lacks.  The first
+        of them that fits goes first; if none does, the latest give their blocks up, and will prefill all of their
+        prompt, until the first request fits."""
+        if self._missing(self.waiting[0]) <= self._unclaimed_blocks():
+            return
+        for i, r in enumerate(self.waiting):
+            if r.blocks and self._missing(r) <= self._unclaimed_blocks():
+                self.waiting.insert(0, self.waiting.pop(i))
+                return
+        for r in [r for r in reversed(self.waiting) if r.blocks]:
+            self.pool.release(r.blocks)
+            r.blocks, r.blocks_np, r.prefilled = [], np.zeros(0, dtype=np.int32), 0
+            if self._missing(self.waiting[0]) <= self._unclaimed_blocks():
+                return
 
     def _chunkable(self, r: Request) -> bool:
         """Whether r's prompt is prefilled in chunks (longer than the prefill budget, attention-only model,
