@@ -76,3 +76,21 @@ def test_a_fork_too_large_for_the_pool_is_refused_when_its_turn_comes():
     assert a in eng.finished
     assert eng.abort_request(b)
     assert eng.pool.free == 7 and not eng.has_work()
+
+
+def test_a_fork_takes_no_block_that_is_promised():
+    """Pipelined steps reach past a request's reservation, so the count of unpromised blocks can fall below zero."""
+    eng = engine(8, method="suffix", seqs=3, asynchronous=True)
+    assert eng._async
+    a = eng.add_request(np.arange(50) % 256, max_new_tokens=70)  # with the look-ahead two blocks to the token
+    b = eng.add_request(np.arange(60) % 256, max_new_tokens=240)  # five blocks in the end
+    while eng._unclaimed_blocks() >= 0:
+        assert a not in eng.finished
+        eng.step()
+    free = eng.pool.free
+    assert free > 0
+    with pytest.raises(MemoryError, match="unpromised"):
+        eng.fork_request(b, max_new_tokens=2)
+    assert a in eng.finished or eng.pool.free == free
+    drain(eng)
+    assert len(eng.finished[b].output) == 240 and eng.pool.free == 7

@@ -305,7 +305,7 @@ class LLMEngine:
         prompt = np.concatenate([parent.prompt, np.asarray(parent.output, dtype=np.int64),
                                  np.asarray(tokens, dtype=np.int64)])
         full, part = divmod(parent.committed, self.block_size)
-        if part and not self._unclaimed_blocks():
+        if part and self._unclaimed_blocks() < 1:  # pipelined steps reach past reservations: it may be negative
             raise MemoryError("no unpromised KV block for the fork's copy of the parent's last block")
         new_rid = self.add_request(prompt, max_new_tokens, new_rid, stop_token_ids)
         r = self.waiting[-1]
