@@ -94,3 +94,27 @@ def test_a_fork_takes_no_block_that_is_promised():
     assert a in eng.finished or eng.pool.free == free
     drain(eng)
     assert len(eng.finished[b].output) == 240 and eng.pool.free == 7
+
+
+# ----------------------------------------------------------------------------------------------- what is copied
+def test_forks_and_compaction_refuse_a_cache_that_is_not_laid_out_by_blocks():
+    """A cache tensor that page copies do not know would keep another request's rows without a word."""
+    eng = engine()
+    a = eng.add_request(np.arange(100) % 256, max_new_tokens=8)
+    b = eng.add_request(np.arange(90) % 256, max_new_tokens=8)
+    eng.step()
+    free = eng.pool.free
+    eng.caches.append((torch.zeros(eng.pool.num_blocks + 1, 64),))
+    with pytest.raises(ValueError, match="laid out by blocks"):
+        eng.fork_request(a, max_new_tokens=2)
+    assert eng.pool.free == free and not eng.waiting
+    eng.caches.pop()
+    eng.fork_request(a, max_new_tokens=2)
+    eng.abort_request(a)
+    eng.caches.append((torch.zeros(eng.pool.num_blocks + 1, 64),))
+    with pytest.raises(ValueError, match="laid out by blocks"):
+        eng.compact_cache()
+    eng.caches.pop()
+    eng.compact_cache()
+    drain(eng)
+    assert len(eng.finished[b].output) == 8

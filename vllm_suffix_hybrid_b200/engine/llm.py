@@ -307,6 +307,7 @@ class LLMEngine:
         full, part = divmod(parent.committed, self.block_size)
         if part and self._unclaimed_blocks() < 1:  # pipelined steps reach past reservations: it may be negative
             raise MemoryError("no unpromised KV block for the fork's copy of the parent's last block")
+        tensors = self._block_tensors()
         new_rid = self.add_request(prompt, max_new_tokens, new_rid, stop_token_ids)
         r = self.waiting[-1]
         shared = parent.blocks[:full]
@@ -315,7 +316,7 @@ class LLMEngine:
         if part:
             own = self.pool.allocate(1)
             ids = torch.tensor([parent.blocks[full], own[0]], device=self.device)
-            ops.copy_kv_pages(self._block_tensors(), ids[:1], ids[1:])
+            ops.copy_kv_pages(tensors, ids[:1], ids[1:])
             r.blocks += own
         r.prefilled = parent.committed
         return new_rid
@@ -338,11 +339,14 @@ class LLMEngine:
         return self.pool.num_blocks - 1 - self.pool.free
 
     def _block_tensors(self) -> List[torch.Tensor]:
-        """Every cache tensor that is laid out by blocks (recurrent states are not)."""
+        """Every paged cache tensor of the target and the draft (recurrent states are objects of their own)."""
         out = []
 
         def walk(x):
             if isinstance(x, torch.Tensor):
+                if x.dim() < 2 or x.shape[0] != self.pool.num_blocks:
+                    raise ValueError(f"a cache tensor of shape {tuple(x.shape)} is not laid out by blocks "
+                                     f"({self.pool.num_blocks} of them)")
                 out.append(x)
             elif isinstance(x, dict):
                 for v in x.values():
@@ -353,7 +357,7 @@ class LLMEngine:
 
         walk(self.caches)
         walk(self.dcaches)
-        return [t for t in out if t.dim() > 1 and t.shape[0] == self.pool.num_blocks]
+        return out
 
     def _fill_caches_random(self, seed: int) -> None:
         gen = torch.Generator(device=self.device).manual_seed(seed) if torch.device(self.device).type == "cuda" \
