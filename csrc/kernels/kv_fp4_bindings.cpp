@@ -207,7 +207,7 @@ void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const
   p.hq = static_cast<int>(hq);
   p.hk = static_cast<int>(hk);
   p.num_blocks = static_cast<int>(k_cache.size(0));
-  p.bt_cols = static_cast<int>(std::min<int64_t>(block_tables.size(1), 1 << 25));
+  p.bt_cols = static_cast<int>(std::min<int64_t>(block_tables.size(1), (1 << 25) - 1));  // positions fit an int
   p.whole_units = invariant ? 1 : 0;
   p.scale_log2 = static_cast<float>(scale * k_scale * kLog2e);
   p.v_scale = static_cast<float>(v_scale);
@@ -225,7 +225,7 @@ void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const
   //     against 39 for 17 tokens at 8000 (2.2M), 32 against 25 for a prompt of 400 (2.9M), 121 against 42 for one of 1000
   //     (16M); 8 heads of 64: 10 against 18 for 400 (1.4M), 29 against 39 for 64 tokens at 12000 (6.2M), 31 against 22 for
   //     1000 (8.2M).
-  const int64_t keys = 64 * p.bt_cols;
+  const int64_t keys = int64_t{64} * p.bt_cols;
   const double work = static_cast<double>(q.size(0)) * static_cast<double>(hq) * static_cast<double>(keys);
   const bool large = d == 128 ? keys > 256 || work > 4e6 : work > (d == 256 ? 2.5e6 : 7.5e6);
   if (rows > (d == 256 ? 48 : 32) && large && !invariant) {

@@ -181,7 +181,7 @@ __device__ __forceinline__ Request request(const AttnFp4Params& p, int b, int ro
   r.q_len = n > 0 ? static_cast<int>(n) : 0;
   int64_t seq = p.seq_lens[b];
   if (seq < 0) seq = 0;
-  const int64_t cap = static_cast<int64_t>(p.bt_cols) * PAGE;  // below 2^31
+  const int64_t cap = static_cast<int64_t>(p.bt_cols) * PAGE;  // below 2^31: bt_cols is at most 2^25 - 1
   r.seq = static_cast<int>(seq < cap ? seq : cap);
   r.tiles = static_cast<int>((static_cast<int64_t>(r.q_len) * (p.hq / p.hk) + rows - 1) / rows);
   r.pages = (r.seq + (PAGE - 1)) / PAGE;
@@ -959,7 +959,7 @@ extern "C" int64_t sh_paged_attention_fp4_workspace(int head_dim, int row_tile) 
 extern "C" int sh_paged_attention_fp4(const AttnFp4Params* params, int head_dim, int row_tile, cudaStream_t stream) {
   const AttnFp4Params& p = *params;
   if (p.num_tokens <= 0 || p.B <= 0) return 0;
-  if (p.hk <= 0 || p.hq % p.hk != 0 || p.num_blocks <= 0 || p.bt_cols <= 0) return -1;
+  if (p.hk <= 0 || p.hq % p.hk != 0 || p.num_blocks <= 0 || p.bt_cols <= 0 || p.bt_cols >= 1 << 25) return -1;
   if (p.part_o == nullptr || p.tickets == nullptr) return -2;
   if ((reinterpret_cast<uintptr_t>(p.k_cache) & 15) || (reinterpret_cast<uintptr_t>(p.v_cache) & 15) ||
       (reinterpret_cast<uintptr_t>(p.q) & 15) || (p.q_stride & 7) || (reinterpret_cast<uintptr_t>(p.out) & 3) ||

@@ -21,7 +21,7 @@ struct AttnFp4Params {
   float* part_o;                 // sh_paged_attention_fp4_workspace floats
   unsigned* tickets;             // zeroed words; every call leaves them zero
   int64_t num_tokens;            // T
-  int B, hq, hk, num_blocks, bt_cols;
+  int B, hq, hk, num_blocks, bt_cols;  // bt_cols: below 2^25, so that a position fits an int
   int whole_units;               // 1: a (request, head, row tile) is never split over CTAs
   float scale_log2;              // softmax scale x log2(e) x the key cache's scale
   float v_scale;                 // the value cache's scale

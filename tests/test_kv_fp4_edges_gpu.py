@@ -58,3 +58,19 @@ def test_branches_of_one_graph_do_not_disturb_each_other(shapes):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+@pytest.mark.parametrize("length", [2 ** 31 - 64, 2 ** 31, 2 ** 40])
+def test_lengths_at_and_beyond_the_widest_table(length):
+    """2^31 positions and more: a length is clipped below 2^31, not wrapped.  Every key is block 0's zero and every value
+    a one, so sums of fewer than 2^24 of them are exact and the result is 1 but for the merges' roundings."""
+    k = torch.zeros(ops.kv_fp4_cache_shape(1, 1, 64), dtype=torch.uint8, device="cuda")
+    v = k.clone()
+    v[..., :32 * 64] = 0x22  # e2m1 1.0, twice
+    v[..., 32 * 64:] = 0x38  # e4m3 1.0
+    q = torch.ones(1, 8 * 64, dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(q, math.nan)
+    bt = torch.zeros(1, 2 ** 25, dtype=torch.int32, device="cuda")
+    ops.paged_attention_fp4(out, q, k, v, bt, torch.tensor([length], device="cuda"), torch.tensor([0, 1], device="cuda"), 8,
+                            64, 0.125, 1)
+    assert (out == 1).all()
