@@ -498,6 +498,9 @@ extern "C" int sh_kv_fp4_write(const KvFp4WriteParams* params, int head_dim, cud
 extern "C" int sh_kv_fp4_read(const KvFp4ReadParams* params, int head_dim, cudaStream_t stream) {
   const KvFp4ReadParams& p = *params;
   if (p.n <= 0) return 0;
+  if ((reinterpret_cast<uintptr_t>(p.k_cache) & 3) || (reinterpret_cast<uintptr_t>(p.v_cache) & 3) ||
+      (reinterpret_cast<uintptr_t>(p.k_out) & 15) || (reinterpret_cast<uintptr_t>(p.v_out) & 15))
+    return -3;
   constexpr int64_t per = READ_THREADS * READ_UNITS;
   const int64_t ctas = (p.n * p.hk * (head_dim / 8) + per - 1) / per;
   if (ctas > 0x7fffffff) return -1;

@@ -74,3 +74,23 @@ def test_lengths_at_and_beyond_the_widest_table(length):
     ops.paged_attention_fp4(out, q, k, v, bt, torch.tensor([length], device="cuda"), torch.tensor([0, 1], device="cuda"), 8,
                             64, 0.125, 1)
     assert (out == 1).all()
+
+
+@pytest.mark.parametrize("off", [1, 2, 4, 8])
+@pytest.mark.parametrize("which", [0, 1])
+def test_caches_that_start_off_16_bytes_are_refused(off, which):
+    """A contiguous view into a larger buffer may start anywhere; every entry point says so before it launches."""
+    shape = ops.kv_fp4_cache_shape(2, 1, 64)
+    n = math.prod(shape)
+    caches = [torch.zeros(shape, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    caches[which] = torch.zeros(n + 16, dtype=torch.uint8, device="cuda")[off:off + n].view(shape)
+    one = torch.zeros(1, dtype=torch.long, device="cuda")
+    q = torch.zeros(1, 3 * 64, dtype=torch.bfloat16, device="cuda")
+    cs = torch.zeros(4, 64, device="cuda")
+    for call in (lambda: ops.kv_fp4_read(*caches, one, 64),
+                 lambda: ops.rope_kv_write_fp4(q, one, cs, *caches, one, 1, 1, 64),
+                 lambda: ops.paged_attention_fp4(torch.empty_like(q), q, *caches, one[None].int(), one,
+                                                 torch.tensor([0, 1], device="cuda"), 1, 64, 0.1, 1),
+                 lambda: ops.copy_kv_pages(caches, one, one + 1)):
+        with pytest.raises(RuntimeError, match="aligned"):
+            call()
