@@ -31,7 +31,7 @@ void check_cache(const torch::Tensor& k, const torch::Tensor& v, int64_t d, cons
                 who, ": caches uint8 [num_blocks, kv_heads, ", page_bytes(d), "] contiguous on a CUDA device");
   for (const torch::Tensor* c : {&k, &v})
     TORCH_CHECK(reinterpret_cast<uintptr_t>(c->data_ptr()) % 16 == 0, who, ": caches must be 16-byte aligned");
-  TORCH_CHECK(k.sizes() == v.sizes(), who, ": key and value caches of one shape");
+  TORCH_CHECK(k.sizes() == v.sizes() && k.device() == v.device(), who, ": key and value caches of one shape on one device");
   TORCH_CHECK(k.size(0) > 0 && k.size(0) <= 0x7fffffff, who, ": 1 .. 2^31 - 1 blocks");
 }
 

@@ -94,3 +94,18 @@ def test_caches_that_start_off_16_bytes_are_refused(off, which):
                  lambda: ops.copy_kv_pages(caches, one, one + 1)):
         with pytest.raises(RuntimeError, match="aligned"):
             call()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_caches_on_two_devices_are_refused():
+    shape = ops.kv_fp4_cache_shape(2, 1, 64)
+    caches = [torch.zeros(shape, dtype=torch.uint8, device=f"cuda:{i}") for i in range(2)]
+    one = torch.zeros(1, dtype=torch.long, device="cuda:0")
+    q = torch.zeros(1, 3 * 64, dtype=torch.bfloat16, device="cuda:0")
+    cs = torch.zeros(4, 64, device="cuda:0")
+    for call in (lambda: ops.kv_fp4_read(*caches, one, 64),
+                 lambda: ops.rope_kv_write_fp4(q, one, cs, *caches, one, 1, 1, 64),
+                 lambda: ops.paged_attention_fp4(torch.empty_like(q), q, *caches, one[None].int(), one,
+                                                 torch.tensor([0, 1], device="cuda:0"), 1, 64, 0.1, 1)):
+        with pytest.raises(RuntimeError, match="one device"):
+            call()
