@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cstdlib>
 #include <map>
 #include <mutex>
@@ -33,6 +34,12 @@ void check_cache(const torch::Tensor& k, const torch::Tensor& v, int64_t d, cons
     TORCH_CHECK(reinterpret_cast<uintptr_t>(c->data_ptr()) % 16 == 0, who, ": caches must be 16-byte aligned");
   TORCH_CHECK(k.sizes() == v.sizes() && k.device() == v.device(), who, ": key and value caches of one shape on one device");
   TORCH_CHECK(k.size(0) > 0 && k.size(0) <= 0x7fffffff, who, ": 1 .. 2^31 - 1 blocks");
+}
+
+// A cache's scale and its reciprocal are kept as normal fp32 numbers.
+void check_scales(double k_scale, double v_scale, const char* who) {
+  for (const double s : {k_scale, v_scale})
+    TORCH_CHECK(s >= FLT_MIN && s <= 1.0 / FLT_MIN, who, ": cache scales must be positive, from 2^-126 to 2^126, got ", s);
 }
 
 void check_index(const torch::Tensor& t, at::ScalarType type, int64_t dim, const torch::Tensor& like, const char* who,
@@ -114,7 +121,7 @@ torch::Tensor rope_kv_write_fp4(const torch::Tensor& qkv, const torch::Tensor& p
   TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 2 && cos_sin.size(1) == rot &&
                   cos_sin.is_contiguous() && cos_sin.device() == k_cache.device() && cos_sin.size(0) > 0,
               who, ": cos_sin must be f32 [positions, rot] contiguous");
-  TORCH_CHECK(k_scale > 0 && v_scale > 0, who, ": cache scales must be positive");
+  check_scales(k_scale, v_scale, who);
   if (qkv.size(0) == 0) return q_out;
   const c10::cuda::CUDAGuard guard(k_cache.device());
   KvFp4WriteParams p{};
@@ -147,6 +154,7 @@ std::tuple<torch::Tensor, torch::Tensor> kv_fp4_read(const torch::Tensor& k_cach
   check_dim(d, who);
   check_cache(k_cache, v_cache, d, who);
   check_index(slots, at::kLong, 1, k_cache, who, "slots");
+  check_scales(k_scale, v_scale, who);
   const c10::cuda::CUDAGuard guard(k_cache.device());
   const auto options = k_cache.options().dtype(at::kBFloat16);
   const torch::Tensor k_out = torch::empty({slots.numel(), k_cache.size(1), d}, options);
@@ -188,7 +196,7 @@ void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const
   TORCH_CHECK(q_start.numel() == B + 1 && block_tables.size(0) == B, who, ": q_start of ", B + 1, " and block_tables of ",
               B, " rows for ", B, " lengths");
   TORCH_CHECK(max_q_len >= 1, who, ": max_q_len must be at least 1");
-  TORCH_CHECK(k_scale > 0 && v_scale > 0, who, ": cache scales must be positive");
+  check_scales(k_scale, v_scale, who);
   if (q.size(0) == 0 || B == 0) return;
   TORCH_CHECK(block_tables.size(1) > 0, who, ": block_tables without columns");
   const c10::cuda::CUDAGuard guard(k_cache.device());

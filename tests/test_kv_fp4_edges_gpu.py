@@ -109,3 +109,19 @@ def test_caches_on_two_devices_are_refused():
                                                  torch.tensor([0, 1], device="cuda:0"), 1, 64, 0.1, 1)):
         with pytest.raises(RuntimeError, match="one device"):
             call()
+
+
+@pytest.mark.parametrize("bad", [0.0, -1.0, math.inf, math.nan, 1e300, 1e-300, 1e-40])
+def test_scales_that_fp32_cannot_hold_are_refused(bad):
+    """An infinite scale made every cached value a zero or a NaN, and one below fp32's range saturated every code."""
+    cache = torch.zeros(ops.kv_fp4_cache_shape(2, 1, 64), dtype=torch.uint8, device="cuda")
+    one = torch.zeros(1, dtype=torch.long, device="cuda")
+    q = torch.zeros(1, 3 * 64, dtype=torch.bfloat16, device="cuda")
+    cs = torch.zeros(4, 64, device="cuda")
+    for gk, gv in ((bad, 1.0), (1.0, bad)):
+        for call in (lambda: ops.kv_fp4_read(cache, cache, one, 64, gk, gv),
+                     lambda: ops.rope_kv_write_fp4(q, one, cs, cache, cache, one, 1, 1, 64, 64, gk, gv),
+                     lambda: ops.paged_attention_fp4(torch.empty_like(q), q, cache, cache, one[None].int(), one,
+                                                     torch.tensor([0, 1], device="cuda"), 1, 64, 0.1, 1, gk, gv)):
+            with pytest.raises(RuntimeError, match="scales"):
+                call()
