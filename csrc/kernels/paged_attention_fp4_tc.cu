@@ -974,7 +974,8 @@ int launch(const AttnFp4Params& p, cudaStream_t st) {
 }  // namespace
 
 extern "C" int64_t sh_paged_attention_fp4_tc_workspace(int head_dim) {
-  return static_cast<int64_t>(num_sms()) * (4 * (head_dim + 2) * 128 + sizeof(Split) / 4);
+  const int query_tiles = head_dim == 256 ? Smem<256>::NQ : Smem<128>::NQ;
+  return static_cast<int64_t>(num_sms()) * (2 * query_tiles * (head_dim + 2) * 128 + sizeof(Split) / 4);
 }
 
 extern "C" int sh_paged_attention_fp4_tc(const AttnFp4Params* params, int head_dim, cudaStream_t stream) {

@@ -125,3 +125,18 @@ def test_scales_that_fp32_cannot_hold_are_refused(bad):
                                                      torch.tensor([0, 1], device="cuda"), 1, 64, 0.1, 1, gk, gv)):
             with pytest.raises(RuntimeError, match="scales"):
                 call()
+
+
+def test_partials_take_what_the_kernel_writes():
+    """Two partials a run of each query tile: one tile of 256 dimensions is as much as two of 128."""
+    import ctypes
+
+    from vllm_suffix_hybrid_b200 import _C
+
+    size = ctypes.CDLL(_C.__file__).sh_paged_attention_fp4_tc_workspace
+    size.restype, size.argtypes = ctypes.c_int64, [ctypes.c_int]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    torch.zeros(1, device="cuda")  # the function asks for the current device
+    for d, tiles in ((64, 2), (128, 2), (256, 1)):
+        partials = sms * 2 * tiles * (d + 2) * 128
+        assert partials < size(d) <= partials + sms * 16
