@@ -94,6 +94,7 @@ class Runner:
         self.h_slots = torch.zeros(B, dtype=torch.long, pin_memory=pin)
         self._tiles: Dict[tuple, tuple] = {}
         self.graphs: Dict[tuple, torch.cuda.CUDAGraph] = {}  # (bucket, verify width) -> graph
+        self._warm: Optional[torch.cuda.Stream] = None  # warm-up runs before a capture
         self.event = torch.cuda.Event() if pin else None
         # Device time of the last decode step (H2D of its inputs .. D2H of its results).
         self.ev0 = torch.cuda.Event(enable_timing=True) if pin else None
@@ -311,7 +312,9 @@ class Runner:
         self.seq[:nb].zero_()
         self.bt[:nb].zero_()
         self.slots[:nb].zero_()
-        s = torch.cuda.Stream()
+        if self._warm is None:  # one for all graphs: kernels keep their scratch by stream
+            self._warm = torch.cuda.Stream()
+        s = self._warm
         s.wait_stream(torch.cuda.current_stream())
         W = self.W if W is None else W
         with torch.cuda.stream(s):
