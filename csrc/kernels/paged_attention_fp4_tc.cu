@@ -243,8 +243,8 @@ __device__ __forceinline__ Request request(const AttnFp4Params& p, int b) {
 // tiles would leave some run in the unit's middle without one, and the merge expects a partial of each.
 template <int ROWS>
 __device__ __forceinline__ int64_t tile_cost(const Request& r, int group, int64_t i) {
-  const int64_t seen = r.ctx * group + (i + 1) * ROWS;
-  return kUnit * group + (seen > 0 ? seen : 0);
+  const int64_t w = (r.ctx + kUnit) * group + (i + 1) * ROWS, least = kUnit * group;
+  return w > least ? w : least;
 }
 template <int ROWS>
 __device__ __forceinline__ int64_t cost(const Request& r, int group, int64_t n) {
@@ -268,10 +268,9 @@ struct Segment {
   bool whole, head;              // all of the unit; its beginning
   bool none;                     // this run has no part in it
 };
-// Walks a CTA's run [pos, end) of the units laid end to end.  Request b begins at `base`; after the first unit, which
-// is searched for, each one follows from the last without a division.
+// Walks a CTA's run [pos, end) of the units laid end to end; each one follows from the last without a division.
 struct Cursor {
-  int64_t pos, end, base;
+  int64_t pos, end, r0;  // r0: what of the first unit lies before the run
   int b, tile, h;
   Request r;
 };
@@ -279,20 +278,9 @@ template <int ROWS>
 __device__ __forceinline__ bool next_segment(const AttnFp4Params& p, Cursor& c, Segment& s) {
   if (c.pos >= c.end) return false;
   const int g = p.hq / p.hk;
-  int64_t r0 = 0;
-  if (c.tile < 0) {
-    const int64_t off = c.pos - c.base;
-    int lo = 0, hi = c.r.tiles - 1;  // the tile that holds `off`: its predecessors cost at most that
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (cost<ROWS>(c.r, g, mid) * p.hk <= off) lo = mid;
-      else hi = mid - 1;
-    }
-    const int64_t in = off - cost<ROWS>(c.r, g, lo) * p.hk, w = tile_cost<ROWS>(c.r, g, lo);
-    c.tile = lo;
-    c.h = static_cast<int>(in / w);
-    r0 = in % w;
-  } else if (++c.h == p.hk) {
+  const int64_t r0 = c.r0;
+  c.r0 = 0;
+  if (++c.h == p.hk) {
     c.h = 0;
     ++c.tile;
     while (c.tile >= c.r.tiles) {
@@ -353,7 +341,6 @@ __device__ __forceinline__ int64_t find_run(const AttnFp4Params& p, int run, int
   if (per < least) per = least;
   cur.pos = per * run;
   cur.end = cur.pos + per < total ? cur.pos + per : total;
-  cur.tile = -1;
   if (cur.pos < cur.end) {
     for (int64_t done = 0, b0 = 0; b0 < p.B; b0 += N) {
       const int64_t w = weight(b0 + threadIdx.x);
@@ -377,8 +364,18 @@ __device__ __forceinline__ int64_t find_run(const AttnFp4Params& p, int run, int
       if (done > cur.pos) break;
     }
     cur.b = start_b;
-    cur.base = start_base;
     cur.r = request<ROWS>(p, cur.b);
+    const int64_t off = cur.pos - start_base;
+    int lo = 0, hi = cur.r.tiles - 1;  // the tile that holds `off`: its predecessors cost at most that
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cost<ROWS>(cur.r, group, mid) * p.hk <= off) lo = mid;
+      else hi = mid - 1;
+    }
+    const int64_t in = off - cost<ROWS>(cur.r, group, lo) * p.hk, w = tile_cost<ROWS>(cur.r, group, lo);
+    cur.tile = lo;
+    cur.h = static_cast<int>(in / w) - 1;  // the cursor stands before it
+    cur.r0 = in % w;
   }
   return per;
 }
