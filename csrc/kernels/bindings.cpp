@@ -31,7 +31,7 @@ std::tuple<torch::Tensor, torch::Tensor> kv_fp4_read(const torch::Tensor& k_cach
 void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const torch::Tensor& k_cache,
                          const torch::Tensor& v_cache, const torch::Tensor& block_tables, const torch::Tensor& seq_lens,
                          const torch::Tensor& q_start, int64_t hq, int64_t d, double scale, int64_t max_q_len,
-                         double k_scale, double v_scale);
+                         double k_scale, double v_scale, const c10::optional<torch::Tensor>& err);
 void copy_kv_pages(const py::list& caches, const torch::Tensor& src, const torch::Tensor& dst);
 void silu_mul(torch::Tensor out, torch::Tensor x);
 void embedding(torch::Tensor out, torch::Tensor ids, torch::Tensor table);
@@ -1103,7 +1103,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope_kv_write", &rope_kv_write);
   m.def("rope_kv_write_fp4", &rope_kv_write_fp4);
   m.def("kv_fp4_read", &kv_fp4_read);
-  m.def("paged_attention_fp4", &paged_attention_fp4);
+  m.def("paged_attention_fp4", &paged_attention_fp4, py::arg("out"), py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("block_tables"), py::arg("seq_lens"), py::arg("q_start"), py::arg("hq"), py::arg("d"), py::arg("scale"),
+        py::arg("max_q_len"), py::arg("k_scale"), py::arg("v_scale"), py::arg("err") = py::none());
   m.def("copy_kv_pages", &copy_kv_pages);
   m.def("silu_mul", &silu_mul);
   m.def("embedding", &embedding);

@@ -179,7 +179,7 @@ std::tuple<torch::Tensor, torch::Tensor> kv_fp4_read(const torch::Tensor& k_cach
 void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const torch::Tensor& k_cache,
                          const torch::Tensor& v_cache, const torch::Tensor& block_tables, const torch::Tensor& seq_lens,
                          const torch::Tensor& q_start, int64_t hq, int64_t d, double scale, int64_t max_q_len,
-                         double k_scale, double v_scale) {
+                         double k_scale, double v_scale, const c10::optional<torch::Tensor>& err) {
   const char* who = "paged_attention_fp4";
   const char* env = std::getenv("SH_BATCH_INVARIANT");
   const bool invariant = env != nullptr && env[0] == '1' && env[1] == 0;
@@ -197,6 +197,8 @@ void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const
               B, " rows for ", B, " lengths");
   TORCH_CHECK(max_q_len >= 1, who, ": max_q_len must be at least 1");
   check_scales(k_scale, v_scale, who);
+  TORCH_CHECK(!err.has_value() || (err->scalar_type() == at::kInt && err->numel() >= 1 && err->device() == k_cache.device()),
+              who, ": err must be int32 on ", k_cache.device());
   if (q.size(0) == 0 || B == 0) return;
   TORCH_CHECK(block_tables.size(1) > 0, who, ": block_tables without columns");
   const c10::cuda::CUDAGuard guard(k_cache.device());
@@ -212,6 +214,7 @@ void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const
   p.bt_stride = block_tables.stride(0);
   p.seq_lens = seq_lens.data_ptr<int64_t>();
   p.q_start = q_start.data_ptr<int64_t>();
+  p.err = err.has_value() ? err->data_ptr<int>() : nullptr;
   p.num_tokens = q.size(0);
   p.B = static_cast<int>(B);
   p.hq = static_cast<int>(hq);

@@ -20,6 +20,7 @@ struct AttnFp4Params {
   const int64_t* q_start;        // [B + 1]
   float* part_o;                 // sh_paged_attention_fp4_workspace floats
   unsigned* tickets;             // zeroed words; every call leaves them zero
+  int* err;                      // optional: the code of the first wait that ran out (the kernel for short queries has none)
   int64_t num_tokens;            // T
   int B, hq, hk, num_blocks, bt_cols;  // bt_cols: below 2^25, so that a position fits an int
   int whole_units;               // 1: a (request, head, row tile) is never split over CTAs

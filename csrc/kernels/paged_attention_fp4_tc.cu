@@ -33,8 +33,9 @@
 // prompt of 4096 with 16 heads of 256 takes 207 us (664 TFLOP/s, 40%): one query tile, whose softmax and products wait
 // for each other.
 //
-// Every wait is bounded (2 s); one that runs out raises the CTA's abort flag, the rows of the CTA's units become NaN,
-// and the CTA drains its MMAs and frees its TMEM before it returns.
+// Every wait is bounded (2 s); one that runs out records 600 + role (1 producers, 2 products, 3 softmax) in *err and
+// raises the CTA's abort flag, the rows of the CTA's units become NaN, and the CTA drains its MMAs and frees its TMEM
+// before it returns.
 #include <float.h>
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -430,6 +431,11 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int group = p.hq / p.hk;
+  auto raise = [&](int role) {  // a wait ran out, here or in the warp whose code stands already
+    if (lane != 0) return;
+    if (p.err != nullptr) atomicCAS(p.err, 0, 600 + role);
+    *abort_flag = 1;
+  };
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&qfull[i], 4);
@@ -562,7 +568,7 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
       now = then;
       then = fetch();
     }
-    if (!ok) *abort_flag = 1;
+    if (!ok) raise(1);
   } else if (warp >= MMA_WARP && warp < MMA_WARP + NQ) {
     // ------------------------------------------------------------------ MMA issuer
     // The whole warp walks the loop, on values that the compiler can see to be uniform, and one elected lane (the same
@@ -632,7 +638,7 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
         }
       }
     }
-    if (!ok) *abort_flag = 1;
+    if (!ok) raise(2);
     if (elect_one()) {
       mma_commit(&drain[q]);
       (void)mbar_wait_drain(&drain[q], 0);
@@ -828,7 +834,7 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
       if (keys) {
         if (ok && !__all_sync(0xffffffffu, mbar_wait(&pvdone[q * 2 + ((ns - 1) & 1)], ((ns - 1) >> 1) & 1, abort_flag)))
           ok = false;
-        if (!ok) *abort_flag = 1;
+        if (!ok) raise(3);
         fence_after();
       }
       if (!ok) l = __uint_as_float(0x7fc00000u);  // a wait ran out: NaN, not numbers

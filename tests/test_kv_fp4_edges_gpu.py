@@ -140,3 +140,22 @@ def test_partials_take_what_the_kernel_writes():
     for d, tiles in ((64, 2), (128, 2), (256, 1)):
         partials = sms * 2 * tiles * (d + 2) * 128
         assert partials < size(d) <= partials + sms * 16
+
+
+def test_the_error_word():
+    """It stays zero where no wait runs out, and has to be an int32 on the caches' device."""
+    c = case((300, 200), (4000, 200), 8, 2, 128, seed=60)
+    dev = {n: c[n].cuda() for n in ("q", "k", "v", "bt", "seqs", "qs")}
+    out = torch.empty_like(dev["q"])
+
+    def call(err):
+        ops.paged_attention_fp4(out, dev["q"], dev["k"], dev["v"], dev["bt"], dev["seqs"], dev["qs"], 8, 128, c["scale"],
+                                c["max_q"], c["gk"], c["gv"], err=err)
+
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    call(err)
+    check(c, out)
+    assert err.item() == 0
+    for bad in (err.long(), err.cpu(), err[:0]):
+        with pytest.raises(RuntimeError, match="err must be"):
+            call(bad)

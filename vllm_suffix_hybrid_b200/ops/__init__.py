@@ -209,20 +209,23 @@ def kv_fp4_read(k_cache, v_cache, slots, d, k_scale: float = 1.0, v_scale: float
 
 
 def paged_attention_fp4(out, q, k_cache, v_cache, block_tables, seq_lens, q_start, hq, d, scale, max_q_len: int,
-                        k_scale: float = 1.0, v_scale: float = 1.0):
+                        k_scale: float = 1.0, v_scale: float = 1.0, err: torch.Tensor | None = None):
     """out[T, hq*D] <- causal attention of q [T, hq*D] over the 4-bit paged cache.
 
     seq_lens [B] counts the new tokens; q_start [B + 1] their rows; max_q_len is the longest of them (it picks the
     kernel's row tile, a smaller number stays correct).  Rows that see no key are zero.  No plan, split count or
     length is needed on the host.  In batch-invariant mode (SH_BATCH_INVARIANT=1) a row's result does not depend on
-    the other rows of the call."""
+    the other rows of the call.
+
+    A wait inside the tensor-core kernel that runs out (2 s) makes its rows NaN and, with err (int32 [1], zero), leaves
+    600 + role there: 1 keys and values, 2 products, 3 softmax."""
     if not _cuda(q):
         t = q.shape[0]
         out.view(t, hq, d).copy_(ref.paged_attention_fp4(q[:, : hq * d].reshape(t, hq, d), k_cache, v_cache, block_tables,
                                                          seq_lens, q_start, hq, d, scale, k_scale, v_scale))
         return out
     native().paged_attention_fp4(out, q, k_cache, v_cache, block_tables, seq_lens, q_start, hq, d, scale, max_q_len,
-                                 k_scale, v_scale)
+                                 k_scale, v_scale, err)
     return out
 
 
