@@ -159,3 +159,103 @@ def test_the_error_word():
     for bad in (err.long(), err.cpu(), err[:0]):
         with pytest.raises(RuntimeError, match="err must be"):
             call(bad)
+
+
+# ----------------------------------------------------------------------------------------------- plans of many rows
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (8, 1, 256), (12, 3, 64)])
+def test_many_strided_rows_and_a_strided_table(hq, hk, d):
+    """Whole and cut units whose rows are columns of wider tensors, over a table with spare columns."""
+    c = case((300, 41, 0, 700), (5000, 41, 7, 900), hq, hk, d, seed=70 + d, cols=4000)
+    T = c["q"].shape[0]
+    wide = torch.randn(T, 2 * hq * d + 64, device="cuda").bfloat16()
+    wide[:, 64:64 + hq * d] = c["q"].cuda()
+    outw = torch.zeros(T, hq * d + 24, dtype=torch.bfloat16, device="cuda")
+    bt = torch.randint(0, 1 << 30, (4, 4007), dtype=torch.int32)
+    bt[:, :4000] = c["bt"]
+    got = outw[:, 16:16 + hq * d]
+    ops.paged_attention_fp4(got, wide[:, 64:64 + hq * d], c["k"].cuda(), c["v"].cuda(), bt.cuda()[:, :4000],
+                            c["seqs"].cuda(), c["qs"].cuda(), hq, d, c["scale"], 700, c["gk"], c["gv"])
+    check(c, got)
+    assert (outw[:, :16] == 0).all() and (outw[:, 16 + hq * d:] == 0).all()
+
+
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (8, 1, 256), (8, 2, 64)])
+def test_a_captured_prompt_follows_its_lengths(hq, hk, d):
+    """The tensor-core kernel and its merge under capture: lengths and tables are read at replay."""
+    c = case((300, 130), (5000, 4000), hq, hk, d, seed=80 + d, cols=4000)
+    dev = {n: c[n].cuda() for n in ("k", "v", "bt", "seqs", "qs", "q")}
+    out = torch.empty_like(dev["q"])
+
+    def call():
+        for _ in range(2):
+            ops.paged_attention_fp4(out, dev["q"], dev["k"], dev["v"], dev["bt"], dev["seqs"], dev["qs"], hq, d, c["scale"],
+                                    300, c["gk"], c["gv"])
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for seqs in ((5000, 4000), (300, 3968), (4999, 130), (64, 200)):
+        c["seqs"] = torch.tensor(seqs)
+        dev["seqs"].copy_(c["seqs"])
+        for _ in range(2):
+            out.fill_(math.nan)
+            graph.replay()
+        torch.cuda.synchronize()
+        check(c, out)
+
+
+def test_prompts_on_two_streams_do_not_disturb_each_other():
+    a, b = case((500, 60), (3000, 6000), 8, 2, 128, seed=90), case((400,), (5000,), 8, 1, 256, seed=91, cols=4000)
+    ra, rb = attend(a), attend(b)
+    check(a, ra)
+    check(b, rb)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(8):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(attend((a, b)[i % 2]))
+    torch.cuda.synchronize()
+    for i, r in enumerate(got):
+        assert torch.equal(r, (ra, rb)[i % 2])
+
+
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (8, 1, 256), (8, 2, 64)])
+def test_bad_block_ids_under_many_rows_stay_in_bounds(hq, hk, d):
+    """Ids outside the cache read block 0, whatever it holds; only the rows that use them are affected."""
+    c = case((200, 150), (3000, 2000), hq, hk, d, seed=100 + d, cols=4000)
+    c["bt"][0, 1], c["bt"][0, 2], c["bt"][0, 46] = 1 << 30, -7, c["k"].shape[0]
+    got = attend(c)
+    c["bt"][0, 1:3] = c["bt"][0, 46] = 0
+    same = attend(c)
+    assert torch.equal(got.view(torch.int16), same.view(torch.int16))
+    check(dict(c, q=c["q"][200:], bt=c["bt"][1:], seqs=c["seqs"][1:], qs=torch.tensor([0, 150])), got[200:])
+
+
+# ----------------------------------------------------------------------------------------------- many requests
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 128), (2, 1, 256), (2, 2, 64)])
+@pytest.mark.parametrize("B", [129, 200, 256, 300, 777])
+def test_more_requests_than_threads(hq, hk, d, B):
+    """A CTA's threads look at the requests in several passes; runs begin in every one of them."""
+    g = torch.Generator().manual_seed(B)
+    seqs = torch.randint(0, 500, (B,), generator=g).tolist()
+    q = torch.randint(0, 4, (B,), generator=g).tolist()
+    q[:90] = [0] * 90 if B > 300 else q[:90]  # a first pass that is almost empty
+    q = [min(a, s) if s else a for a, s in zip(q, seqs)]
+    c = case(q, seqs, hq, hk, d, seed=B + d)
+    got = attend(c)
+    check(c, got)
+    assert torch.equal(got, attend(c))
+
+
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 128), (2, 1, 256), (2, 2, 64)])
+def test_many_requests_of_many_rows(hq, hk, d):
+    """The same for the tensor-core kernel, whose CTAs have 416 to 512 threads."""
+    g = torch.Generator().manual_seed(7)
+    seqs = torch.randint(1, 300, (600,), generator=g).tolist()
+    q = [min(s, 3) for s in seqs]
+    q[550], seqs[550] = 200, 700
+    c = case(q, seqs, hq, hk, d, seed=110 + d, cols=4000)
+    check(c, attend(c))
