@@ -238,6 +238,9 @@ void paged_attention_fp4(const torch::Tensor& out, const torch::Tensor& q, const
   //     against 39 for 17 tokens at 8000 (2.2M), 32 against 25 for a prompt of 400 (2.9M), 121 against 42 for one of 1000
   //     (16M); 8 heads of 64: 10 against 18 for 400 (1.4M), 29 against 39 for 64 tokens at 12000 (6.2M), 31 against 22 for
   //     1000 (8.2M).
+  // Keys are the table's columns, for no length is known on the host.  A table far wider than its lengths, as decode steps
+  // pass, makes short windows of many rows look large: 7 tokens at head_dim 256 over 200 keys take 28 where a tight table
+  // gives 14 (4 requests) and 23 (24 requests); over 1000 keys 34 against 24, and 42 against 42.
   const int64_t keys = int64_t{64} * p.bt_cols;
   const double work = static_cast<double>(q.size(0)) * static_cast<double>(hq) * static_cast<double>(keys);
   const bool large = d == 128 ? keys > 256 || work > 4e6 : work > (d == 256 ? 2.5e6 : 7.5e6);

@@ -20,17 +20,22 @@
 // V^T's pairs of adjacent tokens come from interleaving the nibbles of two tokens' words (a shift and a lop3 per 8
 // codes).  e2m1 -> f16 is exact, and so is the product with the e4m3 scale (at most 6 significant bits, between
 // 2^-10 and 2688).  Q goes to f16 after a multiplication by a power of two per row (its largest element into
-// [2^13, 2^14), which keeps bf16's 8 bits for elements down to 2^-38 of it); the power leaves with the softmax scale.
-// P is rounded to f16: 11 bits, where bf16 would cost as much again as the output's own rounding.
+// [2^13, 2^14), which keeps bf16's 8 bits for elements down to 2^-30 of it; smaller ones lose bits, and below 2^-38 they
+// vanish); the power leaves with the softmax scale.  P is rounded to f16: 11 bits, where bf16 would cost as much again as
+// the output's own rounding.  Against the reference's 1 a weight below 2^-14 has fewer bits, and one below 2^-25 counts in
+// the sum alone.
 //
 // The softmax keeps, per row, a reference m that moves only when a score exceeds it by more than 8 (in log2 units):
 // P <= 2^8 stays far from f16's range, and a chunk costs one vote instead of a reduction over the tokens.
 //
-// What bounds it.  Many keys and 8 rows: memory, behind the decoding (8 requests of 131072 keys, 32 heads of 128, 8 kv
-// heads: 1.18 GB in 228 us, 79% of the copy rate).  Short runs: the way to the first key and the merges, about 10 us of
-// latency around 22 pages (64 requests of 2048: 115 MB in 37 us, 48%; 24 of 4000 at head_dim 256: 40 MB in 23 us, 27%).
-// Wide windows: 255 registers leave two warps a scheduler, which wait for their own results (32 windows of 6 tokens,
-// 24 rows: 233 MB in 96 us, 37%, 43% of the issue slots and 41% of the tensor pipe's cycles).
+// What bounds it (times of a call among others).  Many keys and 8 rows: memory, behind the decoding (8 requests of 131072
+// keys, 32 heads of 128, 8 kv heads: 1.18 GB in 261 us, 69% of the copy rate).  Short runs: the way to the first key and
+// the merges, about 10 us of latency around 22 pages (64 requests of 2048: 115 MB in 36 us, 49%; 24 of 4000 at head_dim
+// 256: 40 MB in 23 us, 27%; 64 of 4096 with 8 heads of 64: 29 MB in 18 us, 24%).  Wide windows: 255 registers leave two
+// warps a scheduler, which wait for their own results (32 windows of 6 tokens, 24 rows: 233 MB in 97 us, 37%, 43% of the
+// issue slots and 41% of the tensor pipe's cycles).
+// Whole units (batch-invariant calls) are never cut: those 8 requests then run on 64 CTAs, in 2260 us, and a prompt of
+// 8192 takes 4000 us here where the tensor-core kernel takes 620.
 //
 // Rows that see no key give 0.  Tokens past the end of a sequence are read (they lie in its last page) with V's
 // scale replaced by 0 and their scores by -inf, so what an earlier owner left there does not matter.
@@ -283,7 +288,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   using K = Cfg<D, NT>;
   constexpr int ROWS = 8 * NT, WARPS = K::WARPS, THREADS = K::THREADS, STAGES = K::STAGES;
   constexpr int CHUNK = K::CHUNK, SUB = K::SUB;
-  constexpr int SCOUT = THREADS - 32;  // the thread that walks the run's units, in a warp that has no queries to convert
+  constexpr int SCOUT = THREADS - 32;  // the thread that walks the run's units: the last warp has the fewest queries to convert
   constexpr int MT = D / 16;  // M tiles of O^T
   constexpr int KW = D / 32;  // words of a key in a thread (D/4 codes), two k-steps each
   constexpr int VW = D / 64;  // words of a value in a thread (D/8 codes), four M tiles each

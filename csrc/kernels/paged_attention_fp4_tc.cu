@@ -22,16 +22,18 @@
 //                    it could have had, and the products run under the other tile's (or buffer's) softmax.
 // TMEM: S_q,b (64 columns each, P in their first 32), O_q (D columns each) from column 256.
 //
-// What bounds it.  No single pipe: a prompt of 8192 with 32 heads of 128 takes 595 us (924 TFLOP/s, 55% of the rate of a
-// large bf16 product), a chunk of 2000 at 32768 keys 995 us (1046 TFLOP/s, 63%), with about half of the issue slots, half
-// of the tensor pipe's cycles and 40% of the special-function unit's.  When the chunk took 1020, it took 808 without the
-// softmax and 1014 without the decoding: the chain S, weights, product of one query tile hides behind the other's only
-// in part.  Registers decide much: with the run's cursor in them, not in shared memory, the two took 615 and 1020.
+// What bounds it.  No single pipe: a prompt of 8192 with 32 heads of 128 takes 626 us (878 TFLOP/s, 53% of the rate of a
+// large bf16 product), a chunk of 2000 at 32768 keys 1088 us (957 TFLOP/s, 57%), calls among others with their merges;
+// a prompt of 4096 has about half of the issue slots, half of the tensor pipe's cycles and 40% of the special-function
+// unit's.  In a probe where the chunk took 1020, it took 808 without the softmax and 1014 without the decoding: the chain
+// S, weights, product of one query tile hides behind the other's only in part.  Registers decide much: with the run's
+// cursor in them, not in shared memory, both took 3% more, and with the search for the first unit in each role's walk a
+// prompt of 4096 with 16 heads of 256 took 212 us, not 199.
 // Tried and slower: 128-key tiles with one S buffer, setmaxnreg splits (1110 us: the producers spill), a third tile's
 // codes in registers (1090), the tile's sum as the sign that the reference must move, in place of its maximum (1081), S
 // of two tiles in one product (1247, where the same code took 1079 with one), results through shared memory (1078).  A
-// prompt of 4096 with 16 heads of 256 takes 207 us (664 TFLOP/s, 40%): one query tile, whose softmax and products wait
-// for each other.
+// prompt of 4096 with 16 heads of 256 takes 199 us (690 TFLOP/s, 41%): one query tile, whose softmax and products wait
+// for each other.  One of 8192 with 8 heads of 64 takes 142 us (485 TFLOP/s, 29%): half the products for each exponential.
 //
 // Every wait is bounded (2 s); one that runs out records 600 + role (1 producers, 2 products, 3 softmax) in *err and
 // raises the CTA's abort flag, the rows of the CTA's units become NaN, and the CTA drains its MMAs and frees its TMEM
@@ -710,7 +712,7 @@ __global__ void __launch_bounds__(Smem<D>::THREADS, 1) attn_fp4_tc_kernel(AttnFp
             top = __reduce_max_sync(0xffffffffu, top);
           } else {
 #pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
           }
           // its largest element goes into [2^13, 2^14); the softmax scale's sign goes with the row (0: a zero row), so
           // that cs > 0 and the largest S is the largest score
