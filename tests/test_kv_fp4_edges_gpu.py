@@ -259,3 +259,41 @@ def test_many_requests_of_many_rows(hq, hk, d):
     q[550], seqs[550] = 200, 700
     c = case(q, seqs, hq, hk, d, seed=110 + d, cols=4000)
     check(c, attend(c))
+
+
+@pytest.mark.parametrize("d,hk", [(64, 8), (128, 8), (256, 4)])
+def test_pages_beyond_four_gigabytes(d, hk):
+    """Blocks whose bytes start beyond 2^32: written, read, attended and copied as those of a small cache, bit for bit."""
+    hq, T = 2 * hk, 700
+    page = hk * ops.kv_fp4_cache_shape(1, hk, d)[2]
+    base = 2 ** 32 // page + 1
+    g = torch.Generator(device="cuda").manual_seed(d)
+    qkv = torch.randn(T, (hq + 2 * hk) * d, device="cuda", generator=g).bfloat16()
+    pos = torch.arange(T, device="cuda")
+    cs = ops.ref.rope_cos_sin(T, d, 10000.0).cuda()
+    got = []
+    for first in (1, base):
+        caches = [torch.zeros(ops.kv_fp4_cache_shape(first + 24, hk, d), dtype=torch.uint8, device="cuda") for _ in range(2)]
+        assert first == 1 or caches[0][first:].data_ptr() - caches[0].data_ptr() > 2 ** 32
+        bt = first + torch.randperm(11, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+        slots = bt[pos // 64] * 64 + pos % 64
+        q = ops.rope_kv_write_fp4(qkv, pos, cs, *caches, slots, hq, hk, d)
+        rows = ops.kv_fp4_read(*caches, slots, d)
+        few = ops.rope_kv_write_fp4(qkv[:5], pos[:5], cs, *caches, slots[:5], hq, hk, d)  # the kernel for few tokens
+        again = ops.kv_fp4_read(*caches, slots, d)
+        ops.copy_kv_pages(caches, bt, bt + 12)
+        copied = ops.kv_fp4_read(*caches, slots + 12 * 64, d)
+        outs = []
+        for n in (1, 6, T):
+            out = torch.full((n, hq * d), math.nan, dtype=torch.bfloat16, device="cuda")
+            for table in (bt, bt + 12):
+                wide = torch.zeros(1, 4000, dtype=torch.int32, device="cuda")
+                wide[0, :11] = table
+                ops.paged_attention_fp4(out, q[-n:], *caches, wide, torch.tensor([T], device="cuda"),
+                                        torch.tensor([0, n], device="cuda"), hq, d, d ** -0.5, n)
+                outs.append(out.clone())
+        assert torch.isfinite(outs[-1]).all() and (outs[-1] != 0).any()
+        got.append([q, few, *rows, *again, *copied, *outs])
+        del caches
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
