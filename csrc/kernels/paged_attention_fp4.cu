@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, (Cfg<D, NT>::CTAS)) attn_
   using K = Cfg<D, NT>;
   constexpr int ROWS = 8 * NT, WARPS = K::WARPS, THREADS = K::THREADS, STAGES = K::STAGES;
   constexpr int CHUNK = K::CHUNK, SUB = K::SUB;
-  constexpr int SCOUT = THREADS - 32;  // the thread that walks the run's units: the last warp has the fewest queries to convert
+  constexpr int SCOUT = THREADS - 32;  // walks the run's units, in the last warp: it has the fewest queries to convert
   constexpr int MT = D / 16;  // M tiles of O^T
   constexpr int KW = D / 32;  // words of a key in a thread (D/4 codes), two k-steps each
   constexpr int VW = D / 64;  // words of a value in a thread (D/8 codes), four M tiles each

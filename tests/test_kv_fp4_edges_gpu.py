@@ -24,8 +24,11 @@ def test_more_new_tokens_than_keys_over_many_runs(q, seq, hq, d):
     assert torch.equal(got, attend(c))
 
 
-@pytest.mark.parametrize("shapes", [(((1,) * 5, (7000,) * 5), ((2,) * 4, (9000,) * 4)),
-                                    (((300,), (9000,)), ((90, 200), (5000, 700))), (((1,) * 5, (7000,) * 5), ((300,), (9000,)))])
+DECODE, VERIFY = ((1,) * 5, (7000,) * 5), ((2,) * 4, (9000,) * 4)
+PROMPT, PROMPTS = ((300,), (9000,)), ((90, 200), (5000, 700))
+
+
+@pytest.mark.parametrize("shapes", [(DECODE, VERIFY), (PROMPT, PROMPTS), (DECODE, PROMPT)])
 def test_branches_of_one_graph_do_not_disturb_each_other(shapes):
     """Calls with cut units on two streams of one capture: each branch has partials and tickets of its own."""
     cases = [case(q, s, 8, 2, 128, seed=50 + i) for i, (q, s) in enumerate(shapes)]
