@@ -78,22 +78,39 @@ def test_a_fork_too_large_for_the_pool_is_refused_when_its_turn_comes():
     assert eng.pool.free == 7 and not eng.has_work()
 
 
-def test_a_fork_takes_no_block_that_is_promised():
-    """Pipelined steps reach past a request's reservation, so the count of unpromised blocks can fall below zero."""
-    eng = engine(8, method="suffix", seqs=3, asynchronous=True)
-    assert eng._async
-    a = eng.add_request(np.arange(50) % 256, max_new_tokens=70)  # with the look-ahead two blocks to the token
-    b = eng.add_request(np.arange(60) % 256, max_new_tokens=240)  # five blocks in the end
-    while eng._unclaimed_blocks() >= 0:
-        assert a not in eng.finished
-        eng.step()
-    free = eng.pool.free
-    assert free > 0
-    with pytest.raises(MemoryError, match="unpromised"):
-        eng.fork_request(b, max_new_tokens=2)
-    assert a in eng.finished or eng.pool.free == free
+@pytest.mark.parametrize("asynchronous", [True, False])
+def test_a_fork_takes_no_block_that_is_promised(asynchronous):
+    """Two requests that fill the pool in the end: at no step is there a block for a fork's copy."""
+    eng = engine(10, method="suffix", seqs=3, asynchronous=asynchronous)
+    a = eng.add_request(np.arange(50) % 256, max_new_tokens=126)  # with the look-ahead three blocks to the token
+    b = eng.add_request(np.arange(60) % 256, max_new_tokens=300)  # six
+    eng.step()
+    parent = next(r for r in eng.running if r.rid == b)
+    while a not in eng.finished:
+        assert eng._unclaimed_blocks() == 0
+        if parent.committed % 64:  # (a whole block is shared, not copied)
+            with pytest.raises(MemoryError, match="unpromised"):
+                eng.fork_request(b, max_new_tokens=2)
+        for _ in range(3):
+            eng.step()
+        eng._drain()
     drain(eng)
-    assert len(eng.finished[b].output) == 240 and eng.pool.free == 7
+    assert len(eng.finished[b].output) == 300 and eng.pool.free == 9
+
+
+@pytest.mark.parametrize("method", ["suffix", "hybrid"])
+def test_pipelined_steps_stay_within_their_reservations(method):
+    """Every length at which the pipeline's look-ahead crosses into a new block, in a pool that the requests fill."""
+    eng = engine(10, method=method, seqs=3, asynchronous=True)
+    assert eng._async
+    rng = np.random.default_rng(4)
+    for n in range(100, 164, 3):
+        ids = [eng.add_request(rng.integers(0, 256, n), max_new_tokens=20) for _ in range(3)]
+        while eng.has_work():
+            eng.step()
+            assert eng._unclaimed_blocks() >= 0
+            assert all(len(r.blocks) <= eng._reservation(r) for r in eng.running)
+        assert all(len(eng.finished[i].output) == 20 for i in ids)
 
 
 # ----------------------------------------------------------------------------------------------- what is copied

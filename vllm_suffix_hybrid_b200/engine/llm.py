@@ -305,7 +305,7 @@ class LLMEngine:
         prompt = np.concatenate([parent.prompt, np.asarray(parent.output, dtype=np.int64),
                                  np.asarray(tokens, dtype=np.int64)])
         full, part = divmod(parent.committed, self.block_size)
-        if part and self._unclaimed_blocks() < 1:  # pipelined steps reach past reservations: it may be negative
+        if part and self._unclaimed_blocks() < 1:
             raise MemoryError("no unpromised KV block for the fork's copy of the parent's last block")
         tensors = self._block_tensors()
         new_rid = self.add_request(prompt, max_new_tokens, new_rid, stop_token_ids)
@@ -604,8 +604,10 @@ class LLMEngine:
 
     def _reservation(self, r: Request) -> int:
         """Blocks request r can ever hold: its prompt and every output token, plus the verify window's
-        look-ahead (the decode step keeps blocks for committed + 2k + 2 positions)."""
-        return blocks_for(len(r.prompt) + r.max_new_tokens + 2 * self.k + 2, self.block_size)
+        look-ahead (the decode step keeps blocks for committed + 2k + 2 positions, a pipelined one for
+        2 * lag more; a request ends before they pass a block table's row)."""
+        n = blocks_for(len(r.prompt) + r.max_new_tokens + 2 * self.k + 2 + 2 * self._lag, self.block_size)
+        return min(n, self.max_blocks_per_seq)
 
     def _missing(self, r: Request) -> int:
         """Blocks of the reservation that r does not hold yet (a fork starts with some)."""
